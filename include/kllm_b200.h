@@ -61,8 +61,10 @@ enum {
   KLLM_B200_FLAG_BAD_POSITION = 2, /* RoPE/KV position outside [0, max_seq) */
   KLLM_B200_FLAG_BAD_SLOT = 4,     /* KV cache slot outside [0, n_slots) */
   KLLM_B200_FLAG_BAD_SEQ_END = 8,  /* select_last_rows end index outside [1, rows] */
-  KLLM_B200_FLAG_TIMEOUT = 16      /* a kernel's bounded wait on its tensor-core work ran out;
+  KLLM_B200_FLAG_TIMEOUT = 16,     /* a kernel's bounded wait on its tensor-core work ran out;
                                       that launch's outputs are incomplete */
+  KLLM_B200_FLAG_BAD_SEQ = 32,     /* paged cache: sequence outside [0, n_seqs) */
+  KLLM_B200_FLAG_BAD_PAGE = 64     /* paged cache: page table entry outside [0, n_pages) */
 };
 
 /* Copies the calling thread's most recent error message into buf (always
@@ -281,6 +283,142 @@ int kllm_b200_attention_head_major(const void* q, const void* k_cache, const voi
                                    int64_t n_kv_heads, int64_t head_dim, int64_t n_slots,
                                    int64_t max_seq, int dtype, void* workspace,
                                    int64_t workspace_bytes, int32_t* err_flags, void* stream);
+
+/* ======================================================================== *
+ *  Paged KV cache: norm + RoPE + append, read back, decode attention        *
+ * ======================================================================== */
+
+/* One layer's paged cache. Pages hold page_size consecutive positions of one
+ * sequence; page_table[seq, p] names the page of positions p * page_size ...
+ * (p + 1) * page_size - 1 of sequence seq. Within a page the layout is
+ * head-major, like the slots of the unpaged cache (which is the special case
+ * page_size = max_seq, page_table[seq, 0] = slot).
+ * cache_dtype F16: rows of head_dim fp16 values; the scales are NULL.
+ * cache_dtype I8: rows of head_dim codes in [-127, 127] and one fp32 scale per
+ * row; the row stands for code * scale.
+ * Limits: head_dim 64 or 128; page_size a power of two, 8 to 2^20;
+ * max_pages * page_size at most 2^30; n_pages below 2^31; pages 16-byte
+ * aligned. Table entries that no call reaches (a sequence's unused tail) may
+ * hold anything. The struct is read during a call only. */
+typedef struct kllm_b200_paged_cache {
+  void* k_pages;             /* [n_pages, n_kv_heads, page_size, head_dim] of cache_dtype */
+  void* v_pages;             /* the same */
+  float* k_scales;           /* [n_pages, n_kv_heads, page_size] (I8) or NULL (F16) */
+  float* v_scales;           /* the same */
+  const int32_t* page_table; /* [n_seqs, max_pages] device */
+  int64_t n_pages, page_size, n_kv_heads, head_dim;
+  int64_t n_seqs, max_pages;
+  int cache_dtype;           /* F16 or I8 */
+} kllm_b200_paged_cache;
+
+/* In all three operators below, token t stands at position positions[t] of
+ * sequence seqs[t] (device int32 arrays of n_tokens). A token at position -1
+ * is padding of a fixed-size batch: nothing is read or written for it except
+ * where the operator says so, and no flag is set. Any other position outside
+ * [0, max_pages * page_size) sets KLLM_B200_FLAG_BAD_POSITION, a sequence
+ * outside [0, n_seqs) KLLM_B200_FLAG_BAD_SEQ, and a page table entry outside
+ * [0, n_pages) that the token needs KLLM_B200_FLAG_BAD_PAGE. */
+
+/* Bias + per-head RMSNorm of q and k + rotate-half RoPE + append to the paged
+ * cache, one launch: the work of kllm_b200_qkv_bias_rope_kv_append
+ * (src/model/llama.cpp:89-114) for a paged cache, with norms of the heads.
+ * For each head x of head_dim values (fp32 throughout, one rounding at the end):
+ *     x += bias                                            (bq, bk, bv; each may be NULL)
+ *     x *= (mean(x^2) + eps)^-1/2 * weight                 (q with q_norm, k with k_norm;
+ *                                                           each may be NULL: no norm)
+ *     q, k: rotated by positions[t] * theta^(-2d/head_dim) (the angle in 64 bits, so far
+ *                                                           positions keep their phase)
+ * q goes to q_out as fp16 (q_out == q rotates in place), k and v to row
+ * positions[t] of sequence seqs[t]. F16 cache: rounded to nearest even. I8
+ * cache: scale = max|x| / 127, code = x / scale rounded to nearest even; a
+ * row whose max|x| is below 2^-60 is stored as zeros with scale 0, a
+ * row with an infinity or NaN as zero codes with scale NaN, so that it reads
+ * back as NaN.
+ *   q [n_tokens, n_heads, head_dim], k and v [n_tokens, n_kv_heads, head_dim]
+ *   fp16, heads contiguous; q_stride, k_stride, v_stride and q_out_stride are
+ *   elements between tokens (views into one packed projection are fine),
+ *   multiples of 8 and at least heads * head_dim; pointers 16-byte aligned.
+ *   Biases of bias_dtype and norm weights [head_dim] of norm_dtype (F16 or
+ *   F32), 16-byte aligned. q_out must be q itself or not overlap q, k or v.
+ * A token that is padding or sets a flag leaves its q_out row and the cache
+ * as they were. The (sequence, position) pairs of one call must be distinct:
+ * two tokens that write one row race. */
+int kllm_b200_qkv_norm_rope_kv_append_paged(
+    const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
+    const void* bq, const void* bk, const void* bv, int bias_dtype, const void* q_norm, const void* k_norm,
+    int norm_dtype, float eps, float theta, const int32_t* positions, const int32_t* seqs, int64_t n_tokens,
+    int64_t n_heads, const kllm_b200_paged_cache* cache, void* q_out, int64_t q_out_stride, int32_t* err_flags,
+    void* stream);
+
+/* Reads rows of the paged cache back as fp16 (I8: code * scale rounded to
+ * nearest even). For token t and kv head h the row of position positions[t]
+ * of sequence seqs[t] goes to
+ *   out_slots == NULL: k_out[t, h, :] of [n_tokens, n_kv_heads, head_dim];
+ *   else: k_out[out_slots[t], h, positions[t], :] of a head-major cache
+ *     [n_out_slots, n_kv_heads, out_max_seq, head_dim], which
+ *     kllm_b200_attention_head_major reads (a prompt's next chunk attends to
+ *     its paged prefix that way).
+ * The same for v. A position at or past out_max_seq sets
+ * KLLM_B200_FLAG_BAD_POSITION, a slot outside [0, n_out_slots)
+ * KLLM_B200_FLAG_BAD_SLOT. Rows of padding or flagged tokens, and all others
+ * of the outputs, stay as they were. Outputs 16-byte aligned. */
+int kllm_b200_kv_read_paged(const kllm_b200_paged_cache* cache, const int32_t* positions, const int32_t* seqs,
+                            int64_t n_tokens, const int32_t* out_slots, int64_t n_out_slots, int64_t out_max_seq,
+                            void* k_out, void* v_out, int32_t* err_flags, void* stream);
+
+/* Attention of single new tokens over the paged cache (the decode form of
+ * kllm_b200_attention_head_major): out[t, h, :] = sum_j p_j * v_j over the
+ * positions j = 0..positions[t] of sequence seqs[t], p = softmax_j(q[t, h, :] .
+ * k_j / sqrt(head_dim)), kv head h / (n_heads / n_kv_heads). Scores, softmax
+ * statistics and sums in fp32; the probabilities enter the product with v as
+ * fp16. q and out fp16 with q_stride and out_stride elements between tokens
+ * (multiples of 8), 16-byte aligned, not overlapping. At most 16 query heads
+ * per kv head. Each token is attended on its own (several tokens of one
+ * sequence are allowed; each reads the sequence's pages again). Rows of
+ * padding or flagged tokens become zeros. A cached row beyond positions[t] is
+ * never used, whatever it holds.
+ * Long sequences of small batches are split over the GPU. workspace (device,
+ * 16-byte aligned) holds the parts; kllm_b200_attention_paged_workspace_bytes
+ * gives its size (0 when none is needed), a smaller or NULL workspace gives
+ * coarser splits, with results that differ by rounding only. It needs no
+ * clearing. Calls that share one workspace must not overlap on the GPU
+ * (graphs captured with the same workspace included). */
+int kllm_b200_attention_paged_workspace_bytes(int64_t n_tokens, int64_t n_heads, const kllm_b200_paged_cache* cache,
+                                              int64_t* bytes);
+int kllm_b200_attention_paged(const void* q, int64_t q_stride, const kllm_b200_paged_cache* cache,
+                              const int32_t* positions, const int32_t* seqs, int64_t n_tokens, int64_t n_heads,
+                              void* out, int64_t out_stride, void* workspace, int64_t workspace_bytes,
+                              int32_t* err_flags, void* stream);
+
+/* ======================================================================== *
+ *  Log probabilities                                                        *
+ * ======================================================================== */
+
+/* What a runner answers with beside the sampled token, from one read of the
+ * logits [rows, vocab] (F16 or F32, row_stride >= vocab elements between
+ * rows, any alignment of the element type). With lse the log of the sum of
+ * exp over the row:
+ *   logprobs[r] = logits[r, tokens[r]] - lse
+ *   ranks[r]    = 1 + the number of logits above that of tokens[r]
+ *   entropies[r] = -sum p log p (natural log)
+ *   top_ids[r, i], top_logprobs[r, i], i < top_k: the top_k largest logits,
+ *     largest first, equal logits in the order of their ids
+ * tokens is a device int32 array; logprobs and ranks must be given with it
+ * (both NULL without it). entropies may be NULL. top_k is 0 to 32 and at most
+ * vocab (top_ids and top_logprobs [rows, top_k], may be NULL when 0). Sums in
+ * fp32. vocab is 1 to 2^30.
+ * tokens[r] == -1 asks for no token: logprobs[r] and ranks[r] are 0. Any other
+ * id outside [0, vocab) gives the same and sets KLLM_B200_FLAG_BAD_TOKEN.
+ * Logits of -inf have probability 0. A row of nothing but -inf has no
+ * distribution: its log probabilities are -inf and its entropy is 0. A row
+ * with a NaN or +inf has NaN log probabilities and entropy; among its top ids
+ * +inf comes first and NaN after all numbers, and its rank counts the logits
+ * that compare above (none against NaN). The sampler that reads such logits
+ * is src/sampler/sampler.cpp:14-98; this operator has no counterpart in the
+ * reference. */
+int kllm_b200_token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, int64_t row_stride,
+                             const int32_t* tokens, float* logprobs, int32_t* ranks, float* entropies, int top_k,
+                             int32_t* top_ids, float* top_logprobs, int32_t* err_flags, void* stream);
 
 /* ======================================================================== *
  *  GEMM with fused epilogues (tcgen05)                                      *

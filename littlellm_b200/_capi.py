@@ -28,6 +28,8 @@ FLAG_BAD_POSITION = 2
 FLAG_BAD_SLOT = 4
 FLAG_BAD_SEQ_END = 8
 FLAG_TIMEOUT = 16
+FLAG_BAD_SEQ = 32
+FLAG_BAD_PAGE = 64
 
 PARAM_IDS = 7680  # host ids carried per launch by kllm_b200_embedding_host_ids
 
@@ -79,6 +81,12 @@ class Chain(ctypes.Structure):
     ]
 
 
+class PagedCache(ctypes.Structure):
+    _fields_ = [(name, ctypes.c_void_p) for name in ("k_pages", "v_pages", "k_scales", "v_scales", "page_table")] + [
+        (name, ctypes.c_int64) for name in ("n_pages", "page_size", "n_kv_heads", "head_dim", "n_seqs", "max_pages")
+    ] + [("cache_dtype", ctypes.c_int)]
+
+
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _i32 = ctypes.c_int32
@@ -118,6 +126,14 @@ SIGNATURES = {
     "kllm_b200_linear_swiglu": [_vp, _vp, _vp, _vp, _vp, _int, _vp, _i64, _i64, _i64, _vp, _vp],
     "kllm_b200_qkv_linear_rope_kv_append": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _int, _vp, _vp, _i64, _i64, _i64,
                                             _i64, _i64, _f32, _vp, _vp, _vp, _i64, _i64, _vp, _vp],
+    "kllm_b200_qkv_norm_rope_kv_append_paged": [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _int, _vp, _vp, _int,
+                                                _f32, _f32, _vp, _vp, _i64, _i64, ctypes.POINTER(PagedCache), _vp,
+                                                _i64, _vp, _vp],
+    "kllm_b200_kv_read_paged": [ctypes.POINTER(PagedCache), _vp, _vp, _i64, _vp, _i64, _i64, _vp, _vp, _vp, _vp],
+    "kllm_b200_attention_paged_workspace_bytes": [_i64, _i64, ctypes.POINTER(PagedCache), ctypes.POINTER(_i64)],
+    "kllm_b200_attention_paged": [_vp, _i64, ctypes.POINTER(PagedCache), _vp, _vp, _i64, _i64, _vp, _i64, _vp, _i64,
+                                  _vp, _vp],
+    "kllm_b200_token_logprobs": [_vp, _int, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp],
     # argtypes of the .kllm entry points use the structures in loader.py
     "kllm_b200_kllm_read_index": None,
     "kllm_b200_kllm_load": None,

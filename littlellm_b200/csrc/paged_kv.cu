@@ -1,0 +1,531 @@
+// paged_kv.cu — writing and reading the paged KV cache (one layer): bias +
+// per-head RMSNorm of q and k + rotate-half RoPE + append in fp16 or int8,
+// and the read back to fp16 rows.
+//
+// Append. Per head x of D values, in fp32 with one rounding at the end:
+//     x += b;  q, k: x *= w / sqrt(mean(x^2) + eps);  q, k: rotate;
+//     q -> fp16;  k, v -> fp16, or scale = max|x| / 127 and
+//     code = rint(x / scale).
+// D / 16 lanes own a head, lane c the elements 8c..8c+7 and D/2 + 8c..+7:
+// both members of its rotation pairs, two 16-byte loads and stores, so the
+// norm's sum and the row's maximum are two or three shuffles and nothing goes
+// through shared memory but the token's cos/sin. A warp covers 32 / (D / 16)
+// heads at a time and U such sets of one token; the inputs of all U are
+// loaded before anything else runs.
+//
+// The angle pos * theta^(-2d/D) is formed in 64 bits and in turns: its
+// fraction is exact to 2^-53 * pos, while an fp32 product would be off by
+// 0.06 rad at position 10^6. The reduced fraction goes to sincospif, which has
+// no slow path.
+//
+// Both kernels are bound by HBM: the append reads T (Hq + 2 Hkv) D fp16 values
+// and writes T Hq D fp16 and 2 T Hkv rows; the read back moves each row once.
+#include <cmath>
+
+#include "paged.cuh"
+
+namespace kb {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kMaxPairs = 64;  // head_dim <= 128
+
+struct AppendArgs {
+  const __half* q;
+  const __half* k;
+  const __half* v;
+  int64_t q_stride, k_stride, v_stride, q_out_stride;
+  const void* bq;
+  const void* bk;
+  const void* bv;
+  const void* q_norm;
+  const void* k_norm;
+  int bias_f32, norm_f32;
+  float eps;
+  const int32_t* positions;
+  const int32_t* seqs;
+  int64_t n_tokens;
+  int n_heads;
+  int warps_per_token;
+  PagedView view;
+  void* k_pages;
+  void* v_pages;
+  float* k_scales;
+  float* v_scales;
+  __half* q_out;
+  int32_t* err_flags;
+  double turns[kMaxPairs];  // theta^(-2d/D) / (2 pi)
+};
+
+// Eight values of a bias or weight vector (fp16 or fp32, 16-byte aligned) from element `at`.
+__device__ __forceinline__ void load8(const void* p, int f32, int at, float (&f)[8]) {
+  if (f32) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at));
+    const float4 y = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(p) + at + 4));
+    f[0] = x.x; f[1] = x.y; f[2] = x.z; f[3] = x.w; f[4] = y.x; f[5] = y.y; f[6] = y.z; f[7] = y.w;
+  } else {
+    unpack8(ld_keep(static_cast<const __half*>(p) + at), f);
+  }
+}
+
+// The larger of two values, NaN when either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// rint(x / scale) as a code in the low byte. inv is 1 / scale rounded, so
+// x * inv is off by up to a step of fp32; one residual step (q += (x - q scale)
+// inv, as in division by a reciprocal) gives the quotient rounded, so a value
+// half way between two codes is seen as such and goes to the even one. Adding
+// 1.5 * 2^23 rounds to a whole number, ties to even.
+__device__ __forceinline__ uint32_t code_of(float x, float scale, float inv) {
+  const float q = x * inv;
+  return __float_as_uint(__fmaf_rn(__fmaf_rn(-q, scale, x), inv, q) + 12582912.f);
+}
+
+// Four codes packed into 32 bits.
+__device__ __forceinline__ uint32_t codes4(const float* x, float scale, float inv) {
+  const uint32_t lo = __byte_perm(code_of(x[0], scale, inv), code_of(x[1], scale, inv), 0x0040);
+  const uint32_t hi = __byte_perm(code_of(x[2], scale, inv), code_of(x[3], scale, inv), 0x0040);
+  return __byte_perm(lo, hi, 0x5410);
+}
+
+template <int D, bool I8, int U>
+__global__ void __launch_bounds__(kThreads) qkv_norm_rope_append_paged_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int L = D / 16;    // lanes of one head
+  constexpr int kSet = 32 / L;  // heads a warp takes at once
+  __shared__ float2 s_cs[kWarps][D / 2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t gw = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
+  const int64_t t = gw / a.warps_per_token;
+  const int part = static_cast<int>(gw - t * a.warps_per_token);
+  grid_dep_wait();
+  grid_dep_launch();
+  if (t >= a.n_tokens) return;  // uniform per warp
+
+  const int hkv = a.view.n_kv_heads;
+  const int n_rows = a.n_heads + 2 * hkv;
+  const int c = lane % L;
+  const int pos = __ldg(a.positions + t), seq = __ldg(a.seqs + t);
+  uint4 lo[U], hi[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int h = (part * U + u) * kSet + lane / L;
+    lo[u] = hi[u] = make_uint4(0u, 0u, 0u, 0u);
+    if (h < n_rows) {
+      const __half* src = h < a.n_heads         ? a.q + t * a.q_stride + h * D
+                          : h < a.n_heads + hkv ? a.k + t * a.k_stride + (h - a.n_heads) * D
+                                                : a.v + t * a.v_stride + (h - a.n_heads - hkv) * D;
+      // coherent loads: with q_out == q this kernel writes what it reads
+      lo[u] = ld_cg(src + 8 * c);
+      hi[u] = ld_cg(src + D / 2 + 8 * c);
+    }
+  }
+  int flag;
+  const TokenState state = token_state(a.view, pos, seq, flag);
+  int page = -1;
+  if (state == kTokenOk) {
+    page = __ldg(a.view.table + seq * a.view.max_pages + (pos >> a.view.page_shift));
+    if (!page_ok(a.view, page)) flag = KLLM_B200_FLAG_BAD_PAGE;
+  }
+  if (state != kTokenOk || flag != 0) {
+    if (flag != 0 && part == 0 && lane == 0) set_flag(a.err_flags, flag);
+    return;
+  }
+#pragma unroll
+  for (int i = lane; i < D / 2; i += 32) {
+    const double w = static_cast<double>(pos) * a.turns[i];
+    const float f = static_cast<float>(w - rint(w));
+    float sn, cs;
+    sincospif(2.f * f, &sn, &cs);
+    s_cs[warp][i] = make_float2(cs, sn);
+  }
+  __syncwarp();
+  const int64_t row0 = ((static_cast<int64_t>(page) * hkv) << a.view.page_shift) + (pos & ((1 << a.view.page_shift) - 1));
+
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int h = (part * U + u) * kSet + lane / L;
+    const bool live = h < n_rows, is_q = h < a.n_heads, is_v = h >= a.n_heads + hkv;
+    const int hh = is_q ? h : is_v ? h - a.n_heads - hkv : h - a.n_heads;  // within its tensor
+    float x[8], y[8], p[8];
+    unpack8(lo[u], x);
+    unpack8(hi[u], y);
+    const void* bias = is_q ? a.bq : is_v ? a.bv : a.bk;
+    if (live && bias != nullptr) {
+      load8(bias, a.bias_f32, hh * D + 8 * c, p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] += p[i];
+      load8(bias, a.bias_f32, hh * D + D / 2 + 8 * c, p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] += p[i];
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
+#pragma unroll
+    for (int m = L / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+    const void* weight = is_v ? nullptr : is_q ? a.q_norm : a.k_norm;
+    if (live && weight != nullptr) {
+      const float r = rsqrtf(ss * (1.f / D) + a.eps);
+      load8(weight, a.norm_f32, 8 * c, p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] *= r * p[i];
+      load8(weight, a.norm_f32, D / 2 + 8 * c, p);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i] *= r * p[i];
+    }
+    if (!is_v) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float2 cs = s_cs[warp][8 * c + i];
+        const float x1 = x[i], x2 = y[i];
+        rope_rotate(x1, x2, cs.x, cs.y, x[i], y[i]);
+      }
+    }
+    if (live && is_q) {
+      __half* dst = a.q_out + t * a.q_out_stride + hh * D + 8 * c;
+      st_plain(dst, pack8(x));
+      st_plain(dst + D / 2, pack8(y));
+    }
+    const int64_t row = row0 + (static_cast<int64_t>(hh) << a.view.page_shift);
+    if (!I8) {
+      if (live && !is_q) {
+        __half* dst = static_cast<__half*>(is_v ? a.v_pages : a.k_pages) + row * D + 8 * c;
+        st_plain(dst, pack8(x));
+        st_plain(dst + D / 2, pack8(y));
+      }
+    } else {
+      float mx = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mx = max_nan(mx, max_nan(fabsf(x[i]), fabsf(y[i])));
+#pragma unroll
+      for (int m = L / 2; m > 0; m >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, m));
+      if (live && !is_q) {
+        // below 2^-60 a row is zero in every use (fp16 ends at 2^-24) and its
+        // reciprocal would leave fp32; an infinity or NaN marks the whole row
+        const bool tiny = mx < 0x1p-60f, sound = mx <= 3.4028235e38f;
+        const float scale = tiny ? 0.f : mx / 127.f;
+        const float inv = tiny || !sound ? 0.f : 1.f / scale;
+        if (!sound) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
+        }
+        int8_t* dst = static_cast<int8_t*>(is_v ? a.v_pages : a.k_pages) + row * D + 8 * c;
+        const float step = sound ? scale : 0.f;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(codes4(x, step, inv), codes4(x + 4, step, inv));
+        *reinterpret_cast<uint2*>(dst + D / 2) = make_uint2(codes4(y, step, inv), codes4(y + 4, step, inv));
+        if (c == 0) (is_v ? a.v_scales : a.k_scales)[row] = sound ? scale : __int_as_float(0x7fffffff);
+      }
+    }
+  }
+}
+
+template <int D, bool I8>
+void (*pick_append(int u))(AppendArgs) {
+  return u == 1 ? qkv_norm_rope_append_paged_kernel<D, I8, 1>
+         : u == 2 ? qkv_norm_rope_append_paged_kernel<D, I8, 2>
+                  : qkv_norm_rope_append_paged_kernel<D, I8, 3>;
+}
+
+// ---------------------------------------------------------------------------
+// Read back
+// ---------------------------------------------------------------------------
+
+constexpr int kReadThreads = 256;
+
+struct ReadArgs {
+  const void* k_pages;
+  const void* v_pages;
+  const float* k_scales;
+  const float* v_scales;
+  PagedView view;
+  const int32_t* positions;
+  const int32_t* seqs;
+  int64_t n_tokens;
+  const int32_t* out_slots;
+  int64_t n_out_slots, out_max_seq;
+  __half* k_out;
+  __half* v_out;
+  int32_t* err_flags;
+};
+
+// Sixteen codes times the row's scale, as fp16.
+__device__ __forceinline__ void dequant16(uint4 w, float scale, uint4& lo, uint4& hi) {
+  const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+  uint32_t h[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int v = static_cast<int>(r[i]);
+    h[2 * i] = f2_to_h2(static_cast<float>(static_cast<int8_t>(v)) * scale,
+                        static_cast<float>(static_cast<int8_t>(v >> 8)) * scale);
+    h[2 * i + 1] = f2_to_h2(static_cast<float>(static_cast<int8_t>(v >> 16)) * scale,
+                            static_cast<float>(static_cast<int8_t>(v >> 24)) * scale);
+  }
+  lo = make_uint4(h[0], h[1], h[2], h[3]);
+  hi = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+// A CTA reads one kv head of a block of consecutive tokens, so consecutive
+// positions are consecutive rows of a page and of a head-major output. A lane
+// takes 16 bytes of a cached row of K and the same of V, of U tokens.
+template <int D, bool I8, int U>
+__global__ void __launch_bounds__(kReadThreads) kv_read_paged_kernel(const __grid_constant__ ReadArgs a) {
+  constexpr int L = I8 ? D / 16 : D / 8;  // lanes of one row
+  constexpr int kRows = kReadThreads / L;
+  grid_dep_wait();
+  grid_dep_launch();
+  const int h = blockIdx.y, hkv = a.view.n_kv_heads;
+  const int c = threadIdx.x % L;
+  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (kRows * U) + threadIdx.x / L;
+  int64_t src[U], dst[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t t = t0 + u * kRows;
+    src[u] = -1;
+    if (t >= a.n_tokens) continue;
+    const int pos = __ldg(a.positions + t), seq = __ldg(a.seqs + t);
+    int flag;
+    const TokenState state = token_state(a.view, pos, seq, flag);
+    if (state == kTokenPadding) continue;
+    int64_t row = t * hkv + h;
+    if (a.out_slots != nullptr) {
+      const int slot = __ldg(a.out_slots + t);
+      if (pos >= a.out_max_seq) flag |= KLLM_B200_FLAG_BAD_POSITION;
+      if (slot < 0 || slot >= a.n_out_slots) flag |= KLLM_B200_FLAG_BAD_SLOT;
+      row = (static_cast<int64_t>(slot) * hkv + h) * a.out_max_seq + pos;
+    }
+    int page = 0;
+    if (state == kTokenOk) {
+      page = __ldg(a.view.table + seq * a.view.max_pages + (pos >> a.view.page_shift));
+      if (!page_ok(a.view, page)) flag |= KLLM_B200_FLAG_BAD_PAGE;
+    }
+    if (flag != 0) {
+      if (h == 0 && c == 0) set_flag(a.err_flags, flag);
+      continue;
+    }
+    dst[u] = row;
+    src[u] = ((static_cast<int64_t>(page) * hkv + h) << a.view.page_shift) + (pos & ((1 << a.view.page_shift) - 1));
+  }
+  uint4 kw[U], vw[U];
+  float ks[U], vs[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (src[u] < 0) continue;
+    const int64_t at = src[u] * (I8 ? D : 2 * D) + 16 * c;
+    kw[u] = ld_stream(static_cast<const char*>(a.k_pages) + at);
+    vw[u] = ld_stream(static_cast<const char*>(a.v_pages) + at);
+    if (I8) {
+      ks[u] = __ldg(a.k_scales + src[u]);
+      vs[u] = __ldg(a.v_scales + src[u]);
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    if (src[u] < 0) continue;
+    if (I8) {
+      uint4 lo, hi;
+      dequant16(kw[u], ks[u], lo, hi);
+      __half* d = a.k_out + dst[u] * D + 16 * c;
+      st_plain(d, lo);
+      st_plain(d + 8, hi);
+      dequant16(vw[u], vs[u], lo, hi);
+      d = a.v_out + dst[u] * D + 16 * c;
+      st_plain(d, lo);
+      st_plain(d + 8, hi);
+    } else {
+      st_plain(a.k_out + dst[u] * D + 8 * c, kw[u]);
+      st_plain(a.v_out + dst[u] * D + 8 * c, vw[u]);
+    }
+  }
+}
+
+template <int D, bool I8, int U>
+int launch_read(const ReadArgs& a, const LaunchOpts& o) {
+  constexpr int kTokens = kReadThreads / (I8 ? D / 16 : D / 8) * U;
+  const int64_t blocks = (a.n_tokens + kTokens - 1) / kTokens;
+  if (blocks > 0x7fffffffLL) return fail(KLLM_B200_ERR_SHAPE, "kv_read_paged: too many tokens");
+  const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.view.n_kv_heads));
+  return launch_status(launch(kv_read_paged_kernel<D, I8, U>, grid, dim3(kReadThreads), 0, o.stream, o.pdl, a),
+                       "kv_read_paged");
+}
+
+}  // namespace
+
+int paged_view(const kllm_b200_paged_cache* c, const char* what, PagedView* v) {
+  if (!c) return fail(KLLM_B200_ERR_INVALID_ARG, "%s: null cache", what);
+  if (c->cache_dtype != KLLM_B200_F16 && c->cache_dtype != KLLM_B200_I8) {
+    return fail(KLLM_B200_ERR_DTYPE, "%s: cache dtype %d not supported (F16, I8)", what, c->cache_dtype);
+  }
+  if (c->n_pages < 0 || c->n_kv_heads < 0 || c->n_seqs < 0 || c->max_pages < 0) {
+    return fail(KLLM_B200_ERR_INVALID_ARG, "%s: negative size", what);
+  }
+  if (c->head_dim != 64 && c->head_dim != 128) {
+    return fail(KLLM_B200_ERR_SHAPE, "%s: head_dim %lld not supported (64, 128)", what, (long long)c->head_dim);
+  }
+  if (c->page_size < 8 || c->page_size > (1LL << 20) || (c->page_size & (c->page_size - 1)) != 0) {
+    return fail(KLLM_B200_ERR_SHAPE, "%s: page_size %lld must be a power of two from 8 to 2^20", what,
+                (long long)c->page_size);
+  }
+  if (c->n_pages == 0 || c->n_kv_heads == 0 || c->n_seqs == 0 || c->max_pages == 0) {
+    return fail(KLLM_B200_ERR_SHAPE, "%s: empty cache", what);
+  }
+  if (c->n_pages > 0x7fffffffLL || c->n_kv_heads > 65535 || c->max_pages > (1LL << 30) / c->page_size ||
+      c->n_seqs > 0x7fffffffLL) {
+    return fail(KLLM_B200_ERR_SHAPE, "%s: cache too large", what);
+  }
+  if (!c->k_pages || !c->v_pages || !c->page_table) return fail(KLLM_B200_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (c->cache_dtype == KLLM_B200_I8 && (!c->k_scales || !c->v_scales)) {
+    return fail(KLLM_B200_ERR_INVALID_ARG, "%s: an I8 cache needs k_scales and v_scales", what);
+  }
+  if (!aligned16(c->k_pages) || !aligned16(c->v_pages)) {
+    return fail(KLLM_B200_ERR_ALIGN, "%s: pages must be 16-byte aligned", what);
+  }
+  v->table = c->page_table;
+  v->max_pages = c->max_pages;
+  v->n_seqs = c->n_seqs;
+  v->n_pages = static_cast<int>(c->n_pages);
+  v->n_kv_heads = static_cast<int>(c->n_kv_heads);
+  v->page_shift = 0;
+  while ((1LL << v->page_shift) < c->page_size) ++v->page_shift;
+  v->capacity = static_cast<int>(c->max_pages * c->page_size);
+  return KLLM_B200_OK;
+}
+
+int qkv_norm_rope_kv_append_paged(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                                  int64_t v_stride, const void* bq, const void* bk, const void* bv, int bias_dtype,
+                                  const void* q_norm, const void* k_norm, int norm_dtype, float eps, float theta,
+                                  const int32_t* positions, const int32_t* seqs, int64_t n_tokens, int64_t n_heads,
+                                  const kllm_b200_paged_cache* cache, void* q_out, int64_t q_out_stride,
+                                  int32_t* err_flags, const LaunchOpts& o) {
+  const char* what = "qkv_norm_rope_kv_append_paged";
+  if (n_tokens < 0 || n_heads < 0) return fail(KLLM_B200_ERR_INVALID_ARG, "%s: negative size", what);
+  AppendArgs a = {};
+  const int rc = paged_view(cache, what, &a.view);
+  if (rc != KLLM_B200_OK) return rc;
+  if (n_tokens == 0) return KLLM_B200_OK;
+  const int64_t D = cache->head_dim, hkv = cache->n_kv_heads;
+  if (n_heads == 0 || n_heads > 65535) return fail(KLLM_B200_ERR_SHAPE, "%s: 1 to 65535 query heads", what);
+  if ((bq || bk || bv) && !is_float_dtype(bias_dtype)) {
+    return fail(KLLM_B200_ERR_DTYPE, "%s: bias dtype %d not supported", what, bias_dtype);
+  }
+  if ((q_norm || k_norm) && !is_float_dtype(norm_dtype)) {
+    return fail(KLLM_B200_ERR_DTYPE, "%s: norm weight dtype %d not supported", what, norm_dtype);
+  }
+  if (!q || !k || !v || !q_out || !positions || !seqs) return fail(KLLM_B200_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (!(theta > 0.f) || !std::isfinite(theta)) return fail(KLLM_B200_ERR_INVALID_ARG, "%s: theta must be positive", what);
+  if (!(eps >= 0.f) || !std::isfinite(eps)) return fail(KLLM_B200_ERR_INVALID_ARG, "%s: eps must not be negative", what);
+  if (q_stride < n_heads * D || q_out_stride < n_heads * D || k_stride < hkv * D || v_stride < hkv * D) {
+    return fail(KLLM_B200_ERR_SHAPE, "%s: a token stride is shorter than the token's row", what);
+  }
+  if (q_out == q && q_out_stride != q_stride) {
+    return fail(KLLM_B200_ERR_SHAPE, "%s: in place, q_out_stride must equal q_stride", what);
+  }
+  if ((q_stride | k_stride | v_stride | q_out_stride) % 8 != 0) {
+    return fail(KLLM_B200_ERR_ALIGN, "%s: token strides must be multiples of 8 elements", what);
+  }
+  for (const void* p : {q, k, v, static_cast<const void*>(q_out), bq, bk, bv, q_norm, k_norm}) {
+    if (!aligned16(p)) return fail(KLLM_B200_ERR_ALIGN, "%s: pointers must be 16-byte aligned", what);
+  }
+  a.q = static_cast<const __half*>(q);
+  a.k = static_cast<const __half*>(k);
+  a.v = static_cast<const __half*>(v);
+  a.q_stride = q_stride;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.q_out_stride = q_out_stride;
+  a.bq = bq;
+  a.bk = bk;
+  a.bv = bv;
+  a.q_norm = q_norm;
+  a.k_norm = k_norm;
+  a.bias_f32 = bias_dtype == KLLM_B200_F32;
+  a.norm_f32 = norm_dtype == KLLM_B200_F32;
+  a.eps = eps;
+  a.positions = positions;
+  a.seqs = seqs;
+  a.n_tokens = n_tokens;
+  a.n_heads = static_cast<int>(n_heads);
+  a.k_pages = cache->k_pages;
+  a.v_pages = cache->v_pages;
+  a.k_scales = cache->k_scales;
+  a.v_scales = cache->v_scales;
+  a.q_out = static_cast<__half*>(q_out);
+  a.err_flags = err_flags;
+  for (int d = 0; d < D / 2; ++d) {
+    a.turns[d] = std::pow(static_cast<double>(theta), -2.0 * d / static_cast<double>(D)) / 6.283185307179586476925;
+  }
+  const int set = static_cast<int>(32 / (D / 16));
+  const int64_t sets = (n_heads + 2 * hkv + set - 1) / set;
+  const int u = 3;
+  a.warps_per_token = static_cast<int>((sets + u - 1) / u);
+  const int64_t warps = n_tokens * a.warps_per_token;
+  if (warps > (int64_t{1} << 32)) return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
+  const unsigned grid = static_cast<unsigned>((warps + kWarps - 1) / kWarps);
+  const bool i8 = cache->cache_dtype == KLLM_B200_I8;
+  void (*kernel)(AppendArgs) = D == 64 ? (i8 ? pick_append<64, true>(u) : pick_append<64, false>(u))
+                                       : (i8 ? pick_append<128, true>(u) : pick_append<128, false>(u));
+  return launch_status(launch(kernel, dim3(grid), dim3(kThreads), 0, o.stream, o.pdl, a), what);
+}
+
+int kv_read_paged(const kllm_b200_paged_cache* cache, const int32_t* positions, const int32_t* seqs, int64_t n_tokens,
+                  const int32_t* out_slots, int64_t n_out_slots, int64_t out_max_seq, void* k_out, void* v_out,
+                  int32_t* err_flags, const LaunchOpts& o) {
+  const char* what = "kv_read_paged";
+  if (n_tokens < 0 || n_out_slots < 0 || out_max_seq < 0) {
+    return fail(KLLM_B200_ERR_INVALID_ARG, "%s: negative size", what);
+  }
+  ReadArgs a = {};
+  const int rc = paged_view(cache, what, &a.view);
+  if (rc != KLLM_B200_OK) return rc;
+  if (n_tokens == 0) return KLLM_B200_OK;
+  if (!positions || !seqs || !k_out || !v_out) return fail(KLLM_B200_ERR_INVALID_ARG, "%s: null pointer", what);
+  if (out_slots && (n_out_slots == 0 || out_max_seq == 0)) return fail(KLLM_B200_ERR_SHAPE, "%s: empty output cache", what);
+  if (!aligned16(k_out) || !aligned16(v_out)) {
+    return fail(KLLM_B200_ERR_ALIGN, "%s: outputs must be 16-byte aligned", what);
+  }
+  a.k_pages = cache->k_pages;
+  a.v_pages = cache->v_pages;
+  a.k_scales = cache->k_scales;
+  a.v_scales = cache->v_scales;
+  a.positions = positions;
+  a.seqs = seqs;
+  a.n_tokens = n_tokens;
+  a.out_slots = out_slots;
+  a.n_out_slots = n_out_slots;
+  a.out_max_seq = out_max_seq;
+  a.k_out = static_cast<__half*>(k_out);
+  a.v_out = static_cast<__half*>(v_out);
+  a.err_flags = err_flags;
+  if (cache->cache_dtype == KLLM_B200_I8) {
+    return cache->head_dim == 64 ? launch_read<64, true, 1>(a, o) : launch_read<128, true, 1>(a, o);
+  }
+  return cache->head_dim == 64 ? launch_read<64, false, 1>(a, o) : launch_read<128, false, 1>(a, o);
+}
+
+}  // namespace kb
+
+extern "C" int kllm_b200_qkv_norm_rope_kv_append_paged(
+    const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride, const void* bq,
+    const void* bk, const void* bv, int bias_dtype, const void* q_norm, const void* k_norm, int norm_dtype, float eps,
+    float theta, const int32_t* positions, const int32_t* seqs, int64_t n_tokens, int64_t n_heads,
+    const kllm_b200_paged_cache* cache, void* q_out, int64_t q_out_stride, int32_t* err_flags, void* stream) {
+  kb::LaunchOpts o;
+  o.stream = static_cast<cudaStream_t>(stream);
+  return kb::qkv_norm_rope_kv_append_paged(q, q_stride, k, k_stride, v, v_stride, bq, bk, bv, bias_dtype, q_norm, k_norm,
+                                           norm_dtype, eps, theta, positions, seqs, n_tokens, n_heads, cache, q_out,
+                                           q_out_stride, err_flags, o);
+}
+
+extern "C" int kllm_b200_kv_read_paged(const kllm_b200_paged_cache* cache, const int32_t* positions,
+                                       const int32_t* seqs, int64_t n_tokens, const int32_t* out_slots,
+                                       int64_t n_out_slots, int64_t out_max_seq, void* k_out, void* v_out,
+                                       int32_t* err_flags, void* stream) {
+  kb::LaunchOpts o;
+  o.stream = static_cast<cudaStream_t>(stream);
+  return kb::kv_read_paged(cache, positions, seqs, n_tokens, out_slots, n_out_slots, out_max_seq, k_out, v_out, err_flags,
+                           o);
+}

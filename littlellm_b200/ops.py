@@ -5,7 +5,9 @@ One function per operator of the reference interface
 add_inplace, select_last_row, silu_mul, rope_inplace, copy_kv_to_cache,
 dequantize_int8) plus the fused/batched entry points (add_rms_norm,
 qkv_bias_rope_kv_append, select_last_rows, attention_head_major, linear,
-linear_swiglu). Each takes CUDA tensors, passes
+linear_swiglu), the operators of a paged cache (PagedKVCache,
+qkv_norm_rope_kv_append_paged, kv_read_paged, attention_paged) and
+token_logprobs. Each takes CUDA tensors, passes
 their device pointers to ``libkllm_b200.so`` on the tensor's current stream
 and raises ``KllmError`` with the library's message on a non-zero status,
 the way the reference throws ``std::runtime_error``.
@@ -14,6 +16,10 @@ torch supplies device memory and streams here; all arithmetic happens in the
 library's kernels.
 """
 from __future__ import annotations
+
+import contextlib
+import ctypes
+from typing import NamedTuple
 
 import torch
 
@@ -416,3 +422,284 @@ def dequantize_int8_batched(data: list[torch.Tensor], scales: list[torch.Tensor]
         check(lib.kllm_b200_dequantize_int8_batched(d_arr, s_arr, o_arr, c_arr, n, out_dtypes.pop(),
                                                     _stream(dev)))
     return outs
+
+
+# ---- paged KV cache ---------------------------------------------------------
+
+
+def _on(device):
+    """The context that makes `device` current; nothing to enter when it is already."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+class PagedKVCache:
+    """One layer's paged KV cache (kllm_b200_paged_cache) over given tensors.
+
+    k_pages and v_pages [n_pages, n_kv_heads, page_size, head_dim], fp16 or
+    int8 (codes; then k_scales and v_scales, fp32 [n_pages, n_kv_heads,
+    page_size], hold the value of one code step per row); page_table int32
+    [n_seqs, max_pages] names the page of each page_size positions of each
+    sequence. head_dim 64 or 128, page_size a power of two of at least 8. The
+    tensors stay the caller's: write page_table in place to hand out pages."""
+
+    def __init__(self, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                 k_scales: torch.Tensor | None = None, v_scales: torch.Tensor | None = None):
+        self.device = _dev(k_pages, v_pages, page_table, k_scales, v_scales)
+        if k_pages.dim() != 4 or v_pages.shape != k_pages.shape or page_table.dim() != 2:
+            raise KllmError(_capi.ERR_SHAPE, "paged cache: k_pages and v_pages [n_pages, n_kv_heads, page_size, "
+                                             "head_dim], page_table [n_seqs, max_pages]")
+        if k_pages.dtype not in (torch.float16, torch.int8) or v_pages.dtype != k_pages.dtype:
+            raise KllmError(_capi.ERR_DTYPE, "paged cache: pages must both be float16 or both int8")
+        if page_table.dtype != torch.int32:
+            raise KllmError(_capi.ERR_DTYPE, "paged cache: page_table must be int32")
+        scales = (k_scales, v_scales)
+        if k_pages.dtype == torch.int8:
+            if any(s is None or s.dtype != torch.float32 for s in scales):
+                raise KllmError(_capi.ERR_DTYPE, "paged cache: int8 pages need float32 k_scales and v_scales")
+            if any(s.shape != k_pages.shape[:3] for s in scales):
+                raise KllmError(_capi.ERR_SHAPE, "paged cache: scales must be [n_pages, n_kv_heads, page_size]")
+        elif any(s is not None for s in scales):
+            raise KllmError(_capi.ERR_INVALID_ARG, "paged cache: float16 pages take no scales")
+        self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
+        self.k_scales, self.v_scales = scales
+
+    @classmethod
+    def allocate(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, n_seqs: int, max_pages: int,
+                 dtype: torch.dtype = torch.float16, device="cuda") -> "PagedKVCache":
+        """An empty cache: zero pages, every table entry -1 (no page)."""
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        pages = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(2)]
+        scales = [torch.zeros(shape[:3], dtype=torch.float32, device=device) if dtype == torch.int8 else None
+                  for _ in range(2)]
+        table = torch.full((n_seqs, max_pages), -1, dtype=torch.int32, device=device)
+        return cls(*pages, table, *scales)
+
+    def descriptor(self) -> _capi.PagedCache:
+        """The C descriptor of the tensors as they are now."""
+        k = self.k_pages
+        n_pages, n_kv_heads, page_size, head_dim = k.shape
+        n_seqs, max_pages = self.page_table.shape
+        return _capi.PagedCache(k.data_ptr(), self.v_pages.data_ptr(), _ptr(self.k_scales), _ptr(self.v_scales),
+                                self.page_table.data_ptr(), n_pages, page_size, n_kv_heads, head_dim, n_seqs,
+                                max_pages, _DTYPES[k.dtype])
+
+
+def _head_rows(x: torch.Tensor, heads: int | None, head_dim: int, what: str) -> int:
+    """Checks x [n_tokens, heads, head_dim] with contiguous heads and returns
+    the elements between its tokens (views into one packed projection pass)."""
+    if not x.is_cuda:
+        raise KllmError(_capi.ERR_INVALID_ARG, "expected a CUDA tensor")
+    if x.dtype != torch.float16:
+        raise KllmError(_capi.ERR_DTYPE, f"{what}: q, k, v and outputs must be float16")
+    if x.dim() != 3 or x.shape[2] != head_dim or (heads is not None and x.shape[1] != heads):
+        raise KllmError(_capi.ERR_SHAPE, f"{what}: expected [n_tokens, heads, {head_dim}], got {tuple(x.shape)}")
+    token, head, element = x.stride()
+    if element != 1 or (head != head_dim and x.shape[1] > 1):
+        raise KllmError(_capi.ERR_SHAPE, f"{what}: the heads of a token must be contiguous")
+    # the stride of a single token is never used
+    return token if x.shape[0] > 1 else max(token, x.shape[1] * head_dim) // 8 * 8
+
+
+def _token_index(x: torch.Tensor, n: int, what: str) -> None:
+    if x.dtype != torch.int32:
+        raise KllmError(_capi.ERR_DTYPE, f"{what}: positions, seqs and slots must be int32")
+    if x.dim() != 1 or x.shape[0] != n:
+        raise KllmError(_capi.ERR_SHAPE, f"{what}: positions, seqs and slots must be [n_tokens]")
+
+
+def _same_device(device, *tensors) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            raise KllmError(_capi.ERR_INVALID_ARG, "tensors are on different devices")
+
+
+def qkv_norm_rope_kv_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache,
+                                  positions: torch.Tensor, seqs: torch.Tensor, theta: float,
+                                  bq: torch.Tensor | None = None, bk: torch.Tensor | None = None,
+                                  bv: torch.Tensor | None = None, q_norm: torch.Tensor | None = None,
+                                  k_norm: torch.Tensor | None = None, eps: float = 1e-6,
+                                  q_out: torch.Tensor | None = None,
+                                  err_flags: torch.Tensor | None = None) -> torch.Tensor:
+    """Bias, per-head RMSNorm of q and k (with the weights q_norm and k_norm
+    [head_dim]; None: no norm) and rotate-half RoPE; k and v are appended to
+    the paged cache at row positions[t] of sequence seqs[t], q goes to q_out
+    (None: rotated in place). q [T, Hq, D], k and v [T, Hkv, D] fp16, tokens
+    at any stride that is a multiple of 8. positions[t] == -1 is padding."""
+    what = "qkv_norm_rope_kv_append_paged"
+    c = cache.descriptor()
+    T, Hq, _ = q.shape if q.dim() == 3 else (0, 0, 0)
+    D, Hkv = c.head_dim, c.n_kv_heads
+    if q_out is None:
+        q_out = q
+    sq, so = _head_rows(q, None, D, what), _head_rows(q_out, Hq, D, what)
+    sk, sv = _head_rows(k, Hkv, D, what), _head_rows(v, Hkv, D, what)
+    if not (k.shape[0] == v.shape[0] == q_out.shape[0] == T):
+        raise KllmError(_capi.ERR_SHAPE, f"{what}: q, k, v and q_out must hold the same number of tokens")
+    _token_index(positions, T, what)
+    _token_index(seqs, T, what)
+    dev = cache.device
+    _dev(positions, seqs, bq, bk, bv, q_norm, k_norm, err_flags)
+    _same_device(dev, q, k, v, q_out, positions, seqs, bq, bk, bv, q_norm, k_norm, err_flags)
+    bias = norm = F16
+    for b, n in ((bq, Hq * D), (bk, Hkv * D), (bv, Hkv * D)):
+        if b is not None:
+            bias = dtype_code(b)
+            if b.numel() != n:
+                raise KllmError(_capi.ERR_SHAPE, f"{what}: a bias must hold heads * head_dim values")
+    for w in (q_norm, k_norm):
+        if w is not None:
+            norm = dtype_code(w)
+            if w.numel() != D:
+                raise KllmError(_capi.ERR_SHAPE, f"{what}: norm weights must hold head_dim values")
+    if len({b.dtype for b in (bq, bk, bv) if b is not None}) > 1 or (
+            q_norm is not None and k_norm is not None and q_norm.dtype != k_norm.dtype):
+        raise KllmError(_capi.ERR_DTYPE, f"{what}: biases must share a dtype, norm weights must share a dtype")
+    with _on(dev):
+        check(lib.kllm_b200_qkv_norm_rope_kv_append_paged(
+            q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, _ptr(bq), _ptr(bk), _ptr(bv), bias, _ptr(q_norm),
+            _ptr(k_norm), norm, eps, theta, positions.data_ptr(), seqs.data_ptr(), T, Hq, c, q_out.data_ptr(), so,
+            _ptr(err_flags), _stream(dev)))
+    return q_out
+
+
+def kv_read_paged(cache: PagedKVCache, positions: torch.Tensor, seqs: torch.Tensor,
+                  k_out: torch.Tensor | None = None, v_out: torch.Tensor | None = None,
+                  out_slots: torch.Tensor | None = None,
+                  err_flags: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """The cached rows at positions[t] of sequences seqs[t] as fp16. Without
+    out_slots: token rows [T, Hkv, D] (allocated as zeros when not given).
+    With out_slots: row positions[t] of slot out_slots[t] of the head-major
+    caches k_out and v_out [n_slots, Hkv, max_seq, D], which
+    attention_head_major reads. Rows of padding (position -1) are not written."""
+    what = "kv_read_paged"
+    c = cache.descriptor()
+    T = positions.numel()
+    _token_index(positions, T, what)
+    _token_index(seqs, T, what)
+    if out_slots is None:
+        shape, n_slots, max_seq = (T, c.n_kv_heads, c.head_dim), 0, 0
+        if k_out is None:
+            k_out = torch.zeros(shape, dtype=torch.float16, device=cache.device)
+        if v_out is None:
+            v_out = torch.zeros(shape, dtype=torch.float16, device=cache.device)
+    else:
+        _token_index(out_slots, T, what)
+        if k_out is None or v_out is None or k_out.dim() != 4:
+            raise KllmError(_capi.ERR_SHAPE, f"{what}: out_slots needs k_out and v_out [n_slots, kv_heads, max_seq, "
+                                             "head_dim]")
+        n_slots, max_seq = k_out.shape[0], k_out.shape[2]
+        shape = (n_slots, c.n_kv_heads, max_seq, c.head_dim)
+    if tuple(k_out.shape) != shape or tuple(v_out.shape) != shape:
+        raise KllmError(_capi.ERR_SHAPE, f"{what}: outputs must be {shape}")
+    if k_out.dtype != torch.float16 or v_out.dtype != torch.float16:
+        raise KllmError(_capi.ERR_DTYPE, f"{what}: outputs must be float16")
+    dev = cache.device
+    _dev(positions, seqs, out_slots, k_out, v_out, err_flags)
+    _same_device(dev, positions, seqs, out_slots, k_out, v_out, err_flags)
+    with _on(dev):
+        check(lib.kllm_b200_kv_read_paged(c, positions.data_ptr(), seqs.data_ptr(), T, _ptr(out_slots), n_slots,
+                                          max_seq, k_out.data_ptr(), v_out.data_ptr(), _ptr(err_flags), _stream(dev)))
+    return k_out, v_out
+
+
+def attention_paged_workspace_bytes(n_tokens: int, n_heads: int, cache: PagedKVCache) -> int:
+    n = ctypes.c_int64(0)
+    with _on(cache.device):
+        check(lib.kllm_b200_attention_paged_workspace_bytes(n_tokens, n_heads, cache.descriptor(), n))
+    return n.value
+
+
+def attention_paged(q: torch.Tensor, cache: PagedKVCache, positions: torch.Tensor, seqs: torch.Tensor,
+                    out: torch.Tensor | None = None, workspace: torch.Tensor | None = None,
+                    err_flags: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of single new tokens over the paged cache: token t sees
+    positions 0..positions[t] of sequence seqs[t]; q and out [T, Hq, D] fp16,
+    tokens at any stride that is a multiple of 8. Padding rows (position -1)
+    become zeros. ``workspace=None`` allocates the preferred one here (the C
+    entry point itself never allocates); it needs no clearing."""
+    what = "attention_paged"
+    c = cache.descriptor()
+    sq = _head_rows(q, None, c.head_dim, what)
+    T, Hq, _ = q.shape
+    if out is None:
+        out = torch.empty((T, Hq, c.head_dim), dtype=q.dtype, device=q.device)
+    so = _head_rows(out, Hq, c.head_dim, what)
+    if out.shape[0] != T:
+        raise KllmError(_capi.ERR_SHAPE, f"{what}: q and out must hold the same number of tokens")
+    _token_index(positions, T, what)
+    _token_index(seqs, T, what)
+    dev = cache.device
+    _dev(positions, seqs, workspace, err_flags)
+    _same_device(dev, q, out, positions, seqs, workspace, err_flags)
+    with _on(dev):
+        if workspace is None:
+            n = ctypes.c_int64(0)
+            check(lib.kllm_b200_attention_paged_workspace_bytes(T, Hq, c, n))
+            if n.value:
+                workspace = torch.empty(n.value, dtype=torch.uint8, device=dev)
+        nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+        check(lib.kllm_b200_attention_paged(q.data_ptr(), sq, c, positions.data_ptr(), seqs.data_ptr(), T, Hq,
+                                            out.data_ptr(), so, _ptr(workspace) if nbytes else None, nbytes,
+                                            _ptr(err_flags), _stream(dev)))
+    return out
+
+
+# ---- log probabilities --------------------------------------------------------
+
+
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs answers for each row of logits."""
+    logprobs: torch.Tensor | None       # fp32 [rows]: log probability of the given token
+    ranks: torch.Tensor | None          # int32 [rows]: 1 + the logits above it
+    entropies: torch.Tensor             # fp32 [rows]
+    top_ids: torch.Tensor | None        # int32 [rows, top_k], most likely first
+    top_logprobs: torch.Tensor | None   # fp32 [rows, top_k]
+
+
+def token_logprobs_buffers(logits: torch.Tensor, top_k: int = 0, tokens: bool = True) -> TokenLogprobs:
+    """Outputs for token_logprobs on logits of this shape."""
+    rows, dev = logits.shape[0], logits.device
+
+    def make(dtype, *shape):
+        return torch.empty(shape, dtype=dtype, device=dev)
+
+    return TokenLogprobs(make(torch.float32, rows) if tokens else None, make(torch.int32, rows) if tokens else None,
+                         make(torch.float32, rows), make(torch.int32, rows, top_k),
+                         make(torch.float32, rows, top_k))
+
+
+def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top_k: int = 0,
+                   out: TokenLogprobs | None = None, err_flags: torch.Tensor | None = None) -> TokenLogprobs:
+    """Log probability and rank of tokens[r] (int32; -1: none asked) under each
+    row of logits [rows, vocab] (fp16 or fp32, rows at any stride), the row's
+    entropy, and its top_k (0 to 32) largest logits as ids and log
+    probabilities, equal logits in the order of their ids."""
+    what = "token_logprobs"
+    if not logits.is_cuda:
+        raise KllmError(_capi.ERR_INVALID_ARG, "expected a CUDA tensor")
+    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+        raise KllmError(_capi.ERR_SHAPE, f"{what}: logits must be [rows, vocab] with contiguous rows")
+    rows, vocab = logits.shape
+    dtype = dtype_code(logits)
+    if out is None:
+        out = token_logprobs_buffers(logits, top_k, tokens is not None)
+    dev = logits.device
+    _dev(tokens, err_flags, *out)
+    _same_device(dev, tokens, err_flags, *out)
+    if tokens is not None:
+        _token_index(tokens, rows, what)
+    if tokens is not None and (out.logprobs is None or out.ranks is None):
+        raise KllmError(_capi.ERR_INVALID_ARG, f"{what}: tokens need logprobs and ranks among the outputs")
+    for t, kind, shape in ((out.logprobs, torch.float32, (rows,)), (out.ranks, torch.int32, (rows,)),
+                           (out.entropies, torch.float32, (rows,)), (out.top_ids, torch.int32, (rows, top_k)),
+                           (out.top_logprobs, torch.float32, (rows, top_k))):
+        if t is not None and (t.dtype != kind or tuple(t.shape) != shape):
+            raise KllmError(_capi.ERR_SHAPE, f"{what}: an output has another shape or dtype than {shape}, {kind}")
+    asked = tokens is not None
+    with _on(dev):
+        check(lib.kllm_b200_token_logprobs(
+            logits.data_ptr(), dtype, rows, vocab, logits.stride(0) if rows > 1 else vocab, _ptr(tokens),
+            _ptr(out.logprobs) if asked else None, _ptr(out.ranks) if asked else None, _ptr(out.entropies), top_k,
+            _ptr(out.top_ids) if top_k else None, _ptr(out.top_logprobs) if top_k else None, _ptr(err_flags),
+            _stream(dev)))
+    return out
