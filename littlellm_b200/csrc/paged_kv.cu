@@ -455,9 +455,10 @@ int qkv_norm_rope_kv_append_paged(const void* q, int64_t q_stride, const void* k
   a.v_scales = cache->v_scales;
   a.q_out = static_cast<__half*>(q_out);
   a.err_flags = err_flags;
-  for (int d = 0; d < D / 2; ++d) {
-    a.turns[d] = std::pow(static_cast<double>(theta), -2.0 * d / static_cast<double>(D)) / 6.283185307179586476925;
-  }
+  // powers by repeated products: 63 roundings of 2^-53 are 10^-8 of a turn at position 10^6
+  const double step = std::pow(static_cast<double>(theta), -2.0 / static_cast<double>(D));
+  a.turns[0] = 1.0 / 6.283185307179586476925;
+  for (int d = 1; d < D / 2; ++d) a.turns[d] = a.turns[d - 1] * step;
   const int set = static_cast<int>(32 / (D / 16));
   const int64_t sets = (n_heads + 2 * hkv + set - 1) / set;
   const int u = 3;

@@ -17,7 +17,6 @@ library's kernels.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 from typing import NamedTuple
 
@@ -59,7 +58,7 @@ def _ptr(t):
 
 
 def _stream(device) -> int:
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def set_pdl(enable: bool) -> bool:
@@ -427,9 +426,23 @@ def dequantize_int8_batched(data: list[torch.Tensor], scales: list[torch.Tensor]
 # ---- paged KV cache ---------------------------------------------------------
 
 
-def _on(device):
-    """The context that makes `device` current; nothing to enter when it is already."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _call(device, entry, *args) -> None:
+    """Calls a C entry point with `device` current (the context is entered only
+    when it is not) and its stream appended, and checks the status."""
+    if device.index == torch.cuda.current_device():
+        check(entry(*args, _stream(device)))
+    else:
+        with torch.cuda.device(device):
+            check(entry(*args, _stream(device)))
+
+
+def _all_on(device, *tensors) -> None:
+    """Checks that every given tensor is contiguous and on `device`."""
+    index = device.index
+    for t in tensors:
+        if t is not None and (t.get_device() != index or not t.is_contiguous()):
+            _dev(t)  # not a CUDA tensor, not contiguous
+            raise KllmError(_capi.ERR_INVALID_ARG, "tensors are on different devices")
 
 
 class PagedKVCache:
@@ -460,8 +473,17 @@ class PagedKVCache:
                 raise KllmError(_capi.ERR_SHAPE, "paged cache: scales must be [n_pages, n_kv_heads, page_size]")
         elif any(s is not None for s in scales):
             raise KllmError(_capi.ERR_INVALID_ARG, "paged cache: float16 pages take no scales")
-        self.k_pages, self.v_pages, self.page_table = k_pages, v_pages, page_table
-        self.k_scales, self.v_scales = scales
+        self._tensors = (k_pages, v_pages, k_scales, v_scales, page_table)
+        n_pages, n_kv_heads, page_size, head_dim = k_pages.shape
+        n_seqs, max_pages = page_table.shape
+        self._descriptor = _capi.PagedCache(None, None, None, None, None, n_pages, page_size, n_kv_heads, head_dim,
+                                            n_seqs, max_pages, dtype_code(k_pages))
+
+    k_pages = property(lambda self: self._tensors[0])
+    v_pages = property(lambda self: self._tensors[1])
+    k_scales = property(lambda self: self._tensors[2])
+    v_scales = property(lambda self: self._tensors[3])
+    page_table = property(lambda self: self._tensors[4])
 
     @classmethod
     def allocate(cls, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, n_seqs: int, max_pages: int,
@@ -475,42 +497,52 @@ class PagedKVCache:
         return cls(*pages, table, *scales)
 
     def descriptor(self) -> _capi.PagedCache:
-        """The C descriptor of the tensors as they are now."""
-        k = self.k_pages
-        n_pages, n_kv_heads, page_size, head_dim = k.shape
-        n_seqs, max_pages = self.page_table.shape
-        return _capi.PagedCache(k.data_ptr(), self.v_pages.data_ptr(), _ptr(self.k_scales), _ptr(self.v_scales),
-                                self.page_table.data_ptr(), n_pages, page_size, n_kv_heads, head_dim, n_seqs,
-                                max_pages, _DTYPES[k.dtype])
+        """The C descriptor (kllm_b200_paged_cache) of the tensors."""
+        d = self._descriptor
+        k, v, ks, vs, table = self._tensors
+        d.k_pages, d.v_pages, d.page_table = k.data_ptr(), v.data_ptr(), table.data_ptr()
+        if ks is not None:
+            d.k_scales, d.v_scales = ks.data_ptr(), vs.data_ptr()
+        return d
 
 
-def _head_rows(x: torch.Tensor, heads: int | None, head_dim: int, what: str) -> int:
-    """Checks x [n_tokens, heads, head_dim] with contiguous heads and returns
-    the elements between its tokens (views into one packed projection pass)."""
-    if not x.is_cuda:
-        raise KllmError(_capi.ERR_INVALID_ARG, "expected a CUDA tensor")
+def _head_rows(x: torch.Tensor, heads: int | None, head_dim: int, device, what: str) -> int:
+    """Checks x [n_tokens, heads, head_dim] on `device`, fp16 with contiguous
+    heads, and returns the elements between its tokens (views into one packed
+    projection pass)."""
+    if x.get_device() != device.index:
+        raise KllmError(_capi.ERR_INVALID_ARG,
+                        "tensors are on different devices" if x.is_cuda else "expected a CUDA tensor")
     if x.dtype != torch.float16:
         raise KllmError(_capi.ERR_DTYPE, f"{what}: q, k, v and outputs must be float16")
-    if x.dim() != 3 or x.shape[2] != head_dim or (heads is not None and x.shape[1] != heads):
-        raise KllmError(_capi.ERR_SHAPE, f"{what}: expected [n_tokens, heads, {head_dim}], got {tuple(x.shape)}")
+    shape = x.shape
+    if len(shape) != 3 or shape[2] != head_dim or (heads is not None and shape[1] != heads):
+        raise KllmError(_capi.ERR_SHAPE, f"{what}: expected [n_tokens, heads, {head_dim}], got {tuple(shape)}")
     token, head, element = x.stride()
-    if element != 1 or (head != head_dim and x.shape[1] > 1):
+    if element != 1 or (head != head_dim and shape[1] > 1):
         raise KllmError(_capi.ERR_SHAPE, f"{what}: the heads of a token must be contiguous")
-    # the stride of a single token is never used
-    return token if x.shape[0] > 1 else max(token, x.shape[1] * head_dim) // 8 * 8
+    return token if shape[0] > 1 else shape[1] * head_dim  # the stride of a single token is never used
 
 
 def _token_index(x: torch.Tensor, n: int, what: str) -> None:
     if x.dtype != torch.int32:
         raise KllmError(_capi.ERR_DTYPE, f"{what}: positions, seqs and slots must be int32")
-    if x.dim() != 1 or x.shape[0] != n:
+    if x.shape != (n,):
         raise KllmError(_capi.ERR_SHAPE, f"{what}: positions, seqs and slots must be [n_tokens]")
 
 
-def _same_device(device, *tensors) -> None:
-    for t in tensors:
-        if t is not None and t.device != device:
-            raise KllmError(_capi.ERR_INVALID_ARG, "tensors are on different devices")
+def _parameters(expected, names: str, what: str) -> int:
+    """Checks optional (tensor, number of values) pairs and returns their dtype's code."""
+    code = None
+    for x, n in expected:
+        if x is None:
+            continue
+        if x.numel() != n:
+            raise KllmError(_capi.ERR_SHAPE, f"{what}: {names} must hold {n} values, got {x.numel()}")
+        if code is not None and code != dtype_code(x):
+            raise KllmError(_capi.ERR_DTYPE, f"{what}: {names} must share a dtype")
+        code = dtype_code(x)
+    return F16 if code is None else code
 
 
 def qkv_norm_rope_kv_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache,
@@ -526,39 +558,24 @@ def qkv_norm_rope_kv_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     (None: rotated in place). q [T, Hq, D], k and v [T, Hkv, D] fp16, tokens
     at any stride that is a multiple of 8. positions[t] == -1 is padding."""
     what = "qkv_norm_rope_kv_append_paged"
-    c = cache.descriptor()
-    T, Hq, _ = q.shape if q.dim() == 3 else (0, 0, 0)
+    c, dev = cache.descriptor(), cache.device
     D, Hkv = c.head_dim, c.n_kv_heads
     if q_out is None:
         q_out = q
-    sq, so = _head_rows(q, None, D, what), _head_rows(q_out, Hq, D, what)
-    sk, sv = _head_rows(k, Hkv, D, what), _head_rows(v, Hkv, D, what)
+    sq = _head_rows(q, None, D, dev, what)
+    T, Hq, _ = q.shape
+    so = sq if q_out is q else _head_rows(q_out, Hq, D, dev, what)
+    sk, sv = _head_rows(k, Hkv, D, dev, what), _head_rows(v, Hkv, D, dev, what)
     if not (k.shape[0] == v.shape[0] == q_out.shape[0] == T):
         raise KllmError(_capi.ERR_SHAPE, f"{what}: q, k, v and q_out must hold the same number of tokens")
     _token_index(positions, T, what)
     _token_index(seqs, T, what)
-    dev = cache.device
-    _dev(positions, seqs, bq, bk, bv, q_norm, k_norm, err_flags)
-    _same_device(dev, q, k, v, q_out, positions, seqs, bq, bk, bv, q_norm, k_norm, err_flags)
-    bias = norm = F16
-    for b, n in ((bq, Hq * D), (bk, Hkv * D), (bv, Hkv * D)):
-        if b is not None:
-            bias = dtype_code(b)
-            if b.numel() != n:
-                raise KllmError(_capi.ERR_SHAPE, f"{what}: a bias must hold heads * head_dim values")
-    for w in (q_norm, k_norm):
-        if w is not None:
-            norm = dtype_code(w)
-            if w.numel() != D:
-                raise KllmError(_capi.ERR_SHAPE, f"{what}: norm weights must hold head_dim values")
-    if len({b.dtype for b in (bq, bk, bv) if b is not None}) > 1 or (
-            q_norm is not None and k_norm is not None and q_norm.dtype != k_norm.dtype):
-        raise KllmError(_capi.ERR_DTYPE, f"{what}: biases must share a dtype, norm weights must share a dtype")
-    with _on(dev):
-        check(lib.kllm_b200_qkv_norm_rope_kv_append_paged(
-            q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv, _ptr(bq), _ptr(bk), _ptr(bv), bias, _ptr(q_norm),
-            _ptr(k_norm), norm, eps, theta, positions.data_ptr(), seqs.data_ptr(), T, Hq, c, q_out.data_ptr(), so,
-            _ptr(err_flags), _stream(dev)))
+    _all_on(dev, positions, seqs, bq, bk, bv, q_norm, k_norm, err_flags)
+    bias = _parameters(((bq, Hq * D), (bk, Hkv * D), (bv, Hkv * D)), "biases", what)
+    norm = _parameters(((q_norm, D), (k_norm, D)), "norm weights", what)
+    _call(dev, lib.kllm_b200_qkv_norm_rope_kv_append_paged, q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv,
+          _ptr(bq), _ptr(bk), _ptr(bv), bias, _ptr(q_norm), _ptr(k_norm), norm, eps, theta, positions.data_ptr(),
+          seqs.data_ptr(), T, Hq, c, q_out.data_ptr(), so, _ptr(err_flags))
     return q_out
 
 
@@ -572,39 +589,36 @@ def kv_read_paged(cache: PagedKVCache, positions: torch.Tensor, seqs: torch.Tens
     caches k_out and v_out [n_slots, Hkv, max_seq, D], which
     attention_head_major reads. Rows of padding (position -1) are not written."""
     what = "kv_read_paged"
-    c = cache.descriptor()
+    c, dev = cache.descriptor(), cache.device
     T = positions.numel()
     _token_index(positions, T, what)
     _token_index(seqs, T, what)
     if out_slots is None:
         shape, n_slots, max_seq = (T, c.n_kv_heads, c.head_dim), 0, 0
         if k_out is None:
-            k_out = torch.zeros(shape, dtype=torch.float16, device=cache.device)
+            k_out = torch.zeros(shape, dtype=torch.float16, device=dev)
         if v_out is None:
-            v_out = torch.zeros(shape, dtype=torch.float16, device=cache.device)
+            v_out = torch.zeros(shape, dtype=torch.float16, device=dev)
     else:
         _token_index(out_slots, T, what)
         if k_out is None or v_out is None or k_out.dim() != 4:
             raise KllmError(_capi.ERR_SHAPE, f"{what}: out_slots needs k_out and v_out [n_slots, kv_heads, max_seq, "
                                              "head_dim]")
-        n_slots, max_seq = k_out.shape[0], k_out.shape[2]
+        n_slots, _, max_seq, _ = k_out.shape
         shape = (n_slots, c.n_kv_heads, max_seq, c.head_dim)
-    if tuple(k_out.shape) != shape or tuple(v_out.shape) != shape:
+    if k_out.shape != shape or v_out.shape != shape:
         raise KllmError(_capi.ERR_SHAPE, f"{what}: outputs must be {shape}")
     if k_out.dtype != torch.float16 or v_out.dtype != torch.float16:
         raise KllmError(_capi.ERR_DTYPE, f"{what}: outputs must be float16")
-    dev = cache.device
-    _dev(positions, seqs, out_slots, k_out, v_out, err_flags)
-    _same_device(dev, positions, seqs, out_slots, k_out, v_out, err_flags)
-    with _on(dev):
-        check(lib.kllm_b200_kv_read_paged(c, positions.data_ptr(), seqs.data_ptr(), T, _ptr(out_slots), n_slots,
-                                          max_seq, k_out.data_ptr(), v_out.data_ptr(), _ptr(err_flags), _stream(dev)))
+    _all_on(dev, positions, seqs, out_slots, k_out, v_out, err_flags)
+    _call(dev, lib.kllm_b200_kv_read_paged, c, positions.data_ptr(), seqs.data_ptr(), T, _ptr(out_slots), n_slots,
+          max_seq, k_out.data_ptr(), v_out.data_ptr(), _ptr(err_flags))
     return k_out, v_out
 
 
 def attention_paged_workspace_bytes(n_tokens: int, n_heads: int, cache: PagedKVCache) -> int:
     n = ctypes.c_int64(0)
-    with _on(cache.device):
+    with torch.cuda.device(cache.device):
         check(lib.kllm_b200_attention_paged_workspace_bytes(n_tokens, n_heads, cache.descriptor(), n))
     return n.value
 
@@ -618,29 +632,25 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, positions: torch.Tenso
     become zeros. ``workspace=None`` allocates the preferred one here (the C
     entry point itself never allocates); it needs no clearing."""
     what = "attention_paged"
-    c = cache.descriptor()
-    sq = _head_rows(q, None, c.head_dim, what)
-    T, Hq, _ = q.shape
+    c, dev = cache.descriptor(), cache.device
+    sq = _head_rows(q, None, c.head_dim, dev, what)
+    T, Hq, D = q.shape
     if out is None:
-        out = torch.empty((T, Hq, c.head_dim), dtype=q.dtype, device=q.device)
-    so = _head_rows(out, Hq, c.head_dim, what)
+        out = torch.empty((T, Hq, D), dtype=q.dtype, device=dev)
+    so = _head_rows(out, Hq, D, dev, what)
     if out.shape[0] != T:
         raise KllmError(_capi.ERR_SHAPE, f"{what}: q and out must hold the same number of tokens")
     _token_index(positions, T, what)
     _token_index(seqs, T, what)
-    dev = cache.device
-    _dev(positions, seqs, workspace, err_flags)
-    _same_device(dev, q, out, positions, seqs, workspace, err_flags)
-    with _on(dev):
-        if workspace is None:
-            n = ctypes.c_int64(0)
-            check(lib.kllm_b200_attention_paged_workspace_bytes(T, Hq, c, n))
-            if n.value:
-                workspace = torch.empty(n.value, dtype=torch.uint8, device=dev)
-        nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-        check(lib.kllm_b200_attention_paged(q.data_ptr(), sq, c, positions.data_ptr(), seqs.data_ptr(), T, Hq,
-                                            out.data_ptr(), so, _ptr(workspace) if nbytes else None, nbytes,
-                                            _ptr(err_flags), _stream(dev)))
+    _all_on(dev, positions, seqs, workspace, err_flags)
+    if workspace is None:
+        nbytes = attention_paged_workspace_bytes(T, Hq, cache)
+        if nbytes:
+            workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    else:
+        nbytes = workspace.numel() * workspace.element_size()
+    _call(dev, lib.kllm_b200_attention_paged, q.data_ptr(), sq, c, positions.data_ptr(), seqs.data_ptr(), T, Hq,
+          out.data_ptr(), so, workspace.data_ptr() if nbytes else None, nbytes, _ptr(err_flags))
     return out
 
 
@@ -675,6 +685,7 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     entropy, and its top_k (0 to 32) largest logits as ids and log
     probabilities, equal logits in the order of their ids."""
     what = "token_logprobs"
+    dev = logits.device
     if not logits.is_cuda:
         raise KllmError(_capi.ERR_INVALID_ARG, "expected a CUDA tensor")
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
@@ -683,23 +694,20 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     dtype = dtype_code(logits)
     if out is None:
         out = token_logprobs_buffers(logits, top_k, tokens is not None)
-    dev = logits.device
-    _dev(tokens, err_flags, *out)
-    _same_device(dev, tokens, err_flags, *out)
+    logprobs, ranks, entropies, top_ids, top_logprobs = out
     if tokens is not None:
         _token_index(tokens, rows, what)
-    if tokens is not None and (out.logprobs is None or out.ranks is None):
-        raise KllmError(_capi.ERR_INVALID_ARG, f"{what}: tokens need logprobs and ranks among the outputs")
-    for t, kind, shape in ((out.logprobs, torch.float32, (rows,)), (out.ranks, torch.int32, (rows,)),
-                           (out.entropies, torch.float32, (rows,)), (out.top_ids, torch.int32, (rows, top_k)),
-                           (out.top_logprobs, torch.float32, (rows, top_k))):
-        if t is not None and (t.dtype != kind or tuple(t.shape) != shape):
+        if logprobs is None or ranks is None:
+            raise KllmError(_capi.ERR_INVALID_ARG, f"{what}: tokens need logprobs and ranks among the outputs")
+    _all_on(dev, tokens, logprobs, ranks, entropies, top_ids, top_logprobs, err_flags)
+    for t, kind, shape in ((logprobs, torch.float32, (rows,)), (ranks, torch.int32, (rows,)),
+                           (entropies, torch.float32, (rows,)), (top_ids, torch.int32, (rows, top_k)),
+                           (top_logprobs, torch.float32, (rows, top_k))):
+        if t is not None and (t.dtype != kind or t.shape != shape):
             raise KllmError(_capi.ERR_SHAPE, f"{what}: an output has another shape or dtype than {shape}, {kind}")
     asked = tokens is not None
-    with _on(dev):
-        check(lib.kllm_b200_token_logprobs(
-            logits.data_ptr(), dtype, rows, vocab, logits.stride(0) if rows > 1 else vocab, _ptr(tokens),
-            _ptr(out.logprobs) if asked else None, _ptr(out.ranks) if asked else None, _ptr(out.entropies), top_k,
-            _ptr(out.top_ids) if top_k else None, _ptr(out.top_logprobs) if top_k else None, _ptr(err_flags),
-            _stream(dev)))
+    _call(dev, lib.kllm_b200_token_logprobs, logits.data_ptr(), dtype, rows, vocab,
+          logits.stride(0) if rows > 1 else vocab, _ptr(tokens), _ptr(logprobs) if asked else None,
+          _ptr(ranks) if asked else None, _ptr(entropies), top_k, _ptr(top_ids) if top_k else None,
+          _ptr(top_logprobs) if top_k else None, _ptr(err_flags))
     return out
