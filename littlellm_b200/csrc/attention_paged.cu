@@ -7,27 +7,38 @@
 // 2 (positions[t] + 1) rows of D fp16 values, or of D codes and a scale, per
 // (token, kv head), and is bound by HBM.
 //
-// A CTA takes one part of the positions of a (token, kv head); its four warps
+// The positions of a (token, kv head) are dealt to the CTAs of a cluster (and,
+// for few tokens over a long cache, to several clusters). A CTA's four warps
 // stream 32-position tiles of K and V through a per-warp cp.async ring, the
-// rows' addresses taken from the page table one tile ahead. Both products run
-// on mma.sync m16n8k16 with the cached rows as the M side: S^T = K Q^T (16
+// rows' addresses taken from the page table one tile ahead; pages hold eight
+// positions at least, so eight rows share one address. Both products run on
+// mma.sync m16n8k16 with the cached rows as the M side: S^T = K Q^T (16
 // positions x 8 heads) and O^T += V^T P^T (16 dims x 8 heads), so a group of up
 // to eight query heads fills the N side; with heads as the M side half or more
 // of every fragment, exponential and accumulator would be padding.
 //
-// int8 rows: a code c becomes the fp16 1024 + (c + 128) by placing its biased
-// byte under the exponent byte 0x64, and one packed subtraction of 1152 leaves
-// c exactly; the scale of a key multiplies its scores, that of a value its
-// probabilities. Codes enter the products exactly.
+// int8 rows. K: the codes go into integer products as they are (mma m16n8k32),
+// with the query head as three int8 digits, q = qmax / (127 2^14) (2^14 h + 2^7 m
+// + l): exact sums of codes with a query that is off by at most 2^-22 of its
+// head's largest value. The key's scale multiplies its scores. V: a code c
+// becomes the fp16 1024 + (c + 128) by placing its byte, top bit flipped, under
+// the exponent byte 0x64 (one logic operation for two codes), and one packed
+// subtraction of 1152 leaves c exactly; the value's scale multiplies its
+// probabilities. (K through the same conversion kept the logic unit at its
+// limit: 214 against 190 us for 2048 sequences of up to 4095 positions.)
 //
-// Softmax: each warp keeps a reference m per head that bounds its scores up to
-// kLag (log2) and the powers 2^(s - m + kLift). Only a tile that exceeds the
-// bound (in practice the first ones) pays for a new maximum and a rescale of
-// the sums. kLift places the largest probabilities near the top of fp16's
-// range, so that those down to 2^-25 of the largest keep 11 bits as operands
-// of the second product; for int8 rows, whose probabilities carry the scale of
-// the value, that scale is taken relative to a power of two at or above the
-// largest the warp has met. Scores, sums and accumulators are fp32.
+// Softmax: each warp keeps a reference m per head and takes the powers
+// 2^(s - m + kLift). Only a tile with a power above kMost (in practice the
+// first one) pays for a new maximum, a rescale of the sums and
+// its powers again. kLift places the largest probabilities near the top of
+// fp16's range, so that those down to 2^-25 of the largest keep 11 bits as
+// operands of the second product; for int8 rows, whose probabilities carry the
+// scale of the value, that scale is taken relative to a power of two at or
+// above the largest the warp has met. Scores, sums and accumulators are fp32.
+//
+// Join: the warps of a CTA through shared memory, the CTAs of a cluster through
+// distributed shared memory (each takes a slice of the output), clusters
+// through the caller's workspace and a second kernel.
 #include <math.h>
 
 #include "paged.cuh"
@@ -39,12 +50,13 @@ namespace {
 constexpr int kWarps = 4;
 constexpr int kThreads = kWarps * 32;
 constexpr int kTile = 32;        // positions per warp tile
-constexpr int kStages = 3;       // tiles of the cp.async ring
+constexpr int kStages = 2;       // tiles of the cp.async ring (3: fewer resident CTAs, 2 to 3% slower)
 constexpr int kMaxGroups = 16;   // query heads per kv head
-constexpr int kMaxSplits = 64;   // parts of one (token, kv head)
+constexpr int kMaxCluster = 8;   // CTAs that join over distributed shared memory
+constexpr int kMaxSplits = 16;   // clusters of one (token, kv head)
 constexpr int kCombineWarps = 4;
-constexpr float kLag = 4.f;      // log2 by which a score may exceed the reference
-constexpr float kLift = 11.f;    // 2^(kLift + kLag) < 65504
+constexpr float kLift = 11.f;    // log2 of the power of a score at the reference
+constexpr float kMost = 32768.f;  // a larger power moves the reference (fp16 ends at 65504)
 
 struct PagedAttnArgs {
   const __half* q;
@@ -60,7 +72,8 @@ struct PagedAttnArgs {
   const int32_t* seqs;
   int64_t n_tokens;
   int n_heads, groups;
-  int splits;
+  int cluster;     // CTAs per cluster
+  int splits;      // clusters per (token, kv head)
   float* part_o;   // [T, Hq, splits, D], sums of p v against the part's own max
   float* part_ml;  // [T, Hq, splits, 2] (max, sum); sum -1: the part met a bad page
   int32_t* err_flags;
@@ -103,13 +116,60 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Codes of bytes (i, j) of `w` (bytes already biased by 128) as an fp16 pair.
-template <int SEL>
+__device__ __forceinline__ void mma16832(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%0,%1,%2,%3};\n"
+      : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// The digits h, m, l of four values x = 2^14 h + 2^7 m + l (|x| <= 127 2^14), a
+// byte of each digit's register per value.
+__device__ __forceinline__ void digits(const float (&x)[4], uint32_t (&w)[3]) {
+  w[0] = w[1] = w[2] = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float h = rintf(x[i] * 0x1p-14f), r = fmaf(h, -0x1p14f, x[i]);
+    const float m = rintf(r * 0x1p-7f), l = rintf(fmaf(m, -0x1p7f, r));
+    w[0] |= (static_cast<uint32_t>(static_cast<int>(h)) & 0xffu) << (8 * i);
+    w[1] |= (static_cast<uint32_t>(static_cast<int>(m)) & 0xffu) << (8 * i);
+    w[2] |= (static_cast<uint32_t>(static_cast<int>(l)) & 0xffu) << (8 * i);
+  }
+}
+
+// The larger of two values, NaN when either is.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Codes of bytes 0 and 2 of `w` as an fp16 pair (bytes 1 and 3: shift by 8).
 __device__ __forceinline__ uint32_t codes_h2(uint32_t w) {
-  const uint32_t x = __byte_perm(w, 0x64646464u, SEL);
   const uint32_t bias = 0x64806480u;  // 1152, 1152
+  const uint32_t x = (w & 0x00ff00ffu) ^ bias;
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&bias));
   return *reinterpret_cast<const uint32_t*>(&r);
+}
+
+// 2^x in one instruction (2 ulp; results below the normal range are 0).
+__device__ __forceinline__ float exp2_approx(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
+}
+// A float in the shared memory of CTA `rank` of the cluster, at this CTA's `local`.
+__device__ __forceinline__ float ld_peer(const float* local, uint32_t rank) {
+  uint32_t at;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(local)), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  return v;
 }
 
 // Byte offset of 16-byte chunk `ch` of row `r` in a tile of ROW-byte rows; the
@@ -128,22 +188,37 @@ struct Ring {
   static constexpr int kBytes = kWarps * kStages * kStageBytes;
 };
 
+// Shared memory of the join, over the idle rings.
+template <int D, int NH>
+struct Join {
+  static constexpr int kHeads = 8 * NH;
+  static constexpr int kRedRow = D + 4;  // padded: eight heads' rows spread over the banks
+  static constexpr int kBytes = (kWarps * kHeads * (kRedRow + 2) + kHeads * (D + 2) + 4) * 4;
+};
+
 // One row's (or part's) share of the joined output: exp2 of its max against the
 // joint max; a part that saw nothing has max -inf and weight 0.
-__device__ __forceinline__ float join_weight(float m, float top) { return m == -INFINITY ? 0.f : exp2f(m - top); }
+__device__ __forceinline__ float join_weight(float m, float top) { return m == -INFINITY ? 0.f : exp2_approx(m - top); }
+
+// Resident CTAs that the registers are held to: int8 rows of 64 codes have the
+// shared memory for five, and want their warps (2048 sequences of up to 4095
+// positions: 201 us, with four 215, with six and their spills 219).
+constexpr int min_ctas(int head_dim, bool i8, int n_heads_8) { return i8 && head_dim == 64 && n_heads_8 == 1 ? 5 : 1; }
 
 template <int D, bool I8, int NH>
-__global__ void __launch_bounds__(kThreads) attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
   using R = Ring<D, I8>;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int s_bad;
   constexpr int kRow = R::kRow;
   constexpr int kChunks = kRow / 16;
-  constexpr int kM = D / 16;  // m16 tiles of O^T over head_dim, k16 steps of K Q^T
+  constexpr int kStep = 32 / kChunks;  // rows the warp's lanes copy at once; divides 8
+  constexpr int kM = D / 16;           // m16 tiles of O^T over head_dim, k16 steps of K Q^T
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
-  const int64_t t = blockIdx.x / a.splits;
-  const int part = static_cast<int>(blockIdx.x - t * a.splits);
+  const int parts = a.splits * a.cluster;
+  const int64_t t = blockIdx.x / parts;
+  const int part = static_cast<int>(blockIdx.x - t * parts);
   const int g = blockIdx.y;
   const int G = a.groups;
   if (threadIdx.x == 0) s_bad = 0;
@@ -153,7 +228,7 @@ __global__ void __launch_bounds__(kThreads) attn_paged_kernel(const __grid_const
   const int pos = a.positions[t], seq = a.seqs[t];
   __half* out_t = a.out + t * a.out_stride + static_cast<int64_t>(g) * G * D;
   int flag;
-  if (token_state(a.view, pos, seq, flag) != kTokenOk) {
+  if (token_state(a.view, pos, seq, flag) != kTokenOk) {  // alike in every CTA of the cluster
     if (part == 0) {
       if (threadIdx.x == 0 && g == 0 && flag != 0) set_flag(a.err_flags, flag);
       for (int i = threadIdx.x; i < G * D / 8; i += kThreads) st_plain(out_t + i * 8, make_uint4(0u, 0u, 0u, 0u));
@@ -162,9 +237,10 @@ __global__ void __launch_bounds__(kThreads) attn_paged_kernel(const __grid_const
   }
   const int n = pos + 1;
   const int all_tiles = (n + kTile - 1) / kTile;
-  const int per_part = (all_tiles + a.splits - 1) / a.splits;
-  const int tile0 = part * per_part;
-  if (tile0 >= all_tiles) return;
+  const int per_part = (all_tiles + parts - 1) / parts;
+  const int cluster_part = part / a.cluster;
+  if (cluster_part * a.cluster * per_part >= all_tiles) return;  // nothing left for this cluster
+  const int tile0 = min(part * per_part, all_tiles);
   const int n_tiles = min(per_part, all_tiles - tile0);
   const int my_tiles = n_tiles > warp ? (n_tiles - warp + kWarps - 1) / kWarps : 0;
 
@@ -178,16 +254,19 @@ __global__ void __launch_bounds__(kThreads) attn_paged_kernel(const __grid_const
     const int j = (tile0 + warp + i * kWarps) * kTile + lane;
     return i < my_tiles && j < n ? __ldg(table + (j >> shift)) : -1;
   };
-  // Copies warp tile i into its stage; rows past the last position are
+  const char* const k_bytes = static_cast<const char*>(a.k_pages);
+  const char* const v_bytes = static_cast<const char*>(a.v_pages);
+  const int lane_row = lane / kChunks, lane_ch = lane % kChunks;
+  // Copies warp tile i into stage `st`; rows past the last position are
   // zero-filled, so no stale bits reach the products.
-  auto issue = [&](int i, int page) {
+  auto issue = [&](int i, int page, int st) {
     if (i < my_tiles) {
       const int j0 = (tile0 + warp + i * kWarps) * kTile;
-      unsigned char* sk = ring + (i % kStages) * R::kStageBytes;
+      unsigned char* sk = ring + st * R::kStageBytes;
       unsigned char* sv = sk + R::kTileBytes;
-      const bool in = j0 + lane < n;
-      if (in && !page_ok(a.view, page)) bad = true;
-      const bool ok = in && page_ok(a.view, page);
+      const bool in = j0 + lane < n, fine = page_ok(a.view, page);
+      bad |= in && !fine;
+      const bool ok = in && fine;
       // row index of this lane's position in K and V (row 0 where there is none)
       const int64_t row =
           ok ? (((static_cast<int64_t>(page) * a.view.n_kv_heads + g) << shift) + ((j0 + lane) & mask)) : 0;
@@ -197,13 +276,20 @@ __global__ void __launch_bounds__(kThreads) attn_paged_kernel(const __grid_const
         cp_async4(smem_u32(ss + lane), a.k_scales + row, ok ? 4 : 0);
         cp_async4(smem_u32(ss + kTile + lane), a.v_scales + row, ok ? 4 : 0);
       }
+      const int64_t row_bytes = row * kRow;
 #pragma unroll
-      for (int it = 0; it < kTile * kChunks / 32; ++it) {
-        const int r = (lane + it * 32) / kChunks, ch = (lane + it * 32) % kChunks;
-        const int64_t off = __shfl_sync(0xffffffffu, row, r) * kRow + ch * 16;
-        const int bytes = (live >> r) & 1 ? 16 : 0;
-        cp_async16(smem_u32(sk + swz<kRow>(r, ch)), static_cast<const char*>(a.k_pages) + off, bytes);
-        cp_async16(smem_u32(sv + swz<kRow>(r, ch)), static_cast<const char*>(a.v_pages) + off, bytes);
+      for (int o = 0; o < kTile / 8; ++o) {
+        // rows 8 o .. 8 o + 7 follow one another in one page (page 0's first rows where there are none)
+        const int64_t off = __shfl_sync(0xffffffffu, row_bytes, 8 * o) + lane_row * kRow + lane_ch * 16;
+        const char* kp = k_bytes + off;
+        const char* vp = v_bytes + off;
+#pragma unroll
+        for (int it = 0; it < 8 / kStep; ++it) {
+          const int r = 8 * o + it * kStep + lane_row;
+          const int bytes = (live >> r) & 1 ? 16 : 0;
+          cp_async16(smem_u32(sk + swz<kRow>(r, lane_ch)), kp + it * kStep * kRow, bytes);
+          cp_async16(smem_u32(sv + swz<kRow>(r, lane_ch)), vp + it * kStep * kRow, bytes);
+        }
       }
     }
     cp_async_commit();  // empty groups keep the count uniform
@@ -214,30 +300,66 @@ __global__ void __launch_bounds__(kThreads) attn_paged_kernel(const __grid_const
 #pragma unroll
     for (int i = 0; i < kStages - 1; ++i) first[i] = page_of(i);
 #pragma unroll
-    for (int i = 0; i < kStages - 1; ++i) issue(i, first[i]);
+    for (int i = 0; i < kStages - 1; ++i) issue(i, first[i], i);
   }
   int next_page = page_of(kStages - 1);
 
-  // B fragments of Q^T. int8: lane tig holds dims 4 tig .. 4 tig + 3 of each 16
-  // (the bytes ldmatrix hands it), so the k index is permuted alike on both sides.
-  uint32_t qb[NH][kM][2];
+  // B fragments of Q^T: fp16 pairs, or (int8) the three digits of four dims
+  // each, with what takes a head's integer sums back to its scale.
+  constexpr int kQ = I8 ? D / 32 : kM;  // k steps of K Q^T
+  uint32_t qb[NH][kQ][2][I8 ? 3 : 1];
+  float unit[NH][2];
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
     const int head = h * 8 + gid;
-    const __half* qh = a.q + t * a.q_stride + (static_cast<int64_t>(g) * G + (head < G ? head : 0)) * D;
+    const bool live = head < G;
+    const __half* qh = a.q + t * a.q_stride + (static_cast<int64_t>(g) * G + (live ? head : 0)) * D;
+    if constexpr (!I8) {
 #pragma unroll
-    for (int ks = 0; ks < kM; ++ks) {
-      const int d0 = ks * 16 + (I8 ? 4 : 2) * tig;
-      qb[h][ks][0] = head < G ? *reinterpret_cast<const uint32_t*>(qh + d0) : 0u;
-      qb[h][ks][1] = head < G ? *reinterpret_cast<const uint32_t*>(qh + d0 + (I8 ? 2 : 8)) : 0u;
+      for (int ks = 0; ks < kQ; ++ks) {
+        qb[h][ks][0][0] = live ? *reinterpret_cast<const uint32_t*>(qh + ks * 16 + 2 * tig) : 0u;
+        qb[h][ks][1][0] = live ? *reinterpret_cast<const uint32_t*>(qh + ks * 16 + 2 * tig + 8) : 0u;
+      }
+    } else {
+      uint2 raw[kQ][2];
+      float qmax = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < kQ; ++ks) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          raw[ks][e] = live ? *reinterpret_cast<const uint2*>(qh + ks * 32 + 16 * e + 4 * tig) : make_uint2(0u, 0u);
+          const float2 x = h2_to_f2(raw[ks][e].x), y = h2_to_f2(raw[ks][e].y);
+          qmax = max_nan(qmax, max_nan(max_nan(fabsf(x.x), fabsf(x.y)), max_nan(fabsf(y.x), fabsf(y.y))));
+        }
+      }
+      qmax = max_nan(qmax, __shfl_xor_sync(0xffffffffu, qmax, 1));
+      qmax = max_nan(qmax, __shfl_xor_sync(0xffffffffu, qmax, 2));
+      const float inv = qmax > 0.f ? 2080768.f / qmax : 0.f;  // 127 * 2^14
+#pragma unroll
+      for (int ks = 0; ks < kQ; ++ks) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 x = h2_to_f2(raw[ks][e].x), y = h2_to_f2(raw[ks][e].y);
+          const float v[4] = {x.x * inv, x.y * inv, y.x * inv, y.y * inv};
+          digits(v, qb[h][ks][e]);
+        }
+      }
+      // the heads of this lane's scores are 2 tig and 2 tig + 1; an infinite or
+      // NaN query makes the unit, and with it every score, NaN
+      const float u = qmax * (a.scale_log2 / 2080768.f) * (qmax <= 65504.f ? 1.f : __int_as_float(0x7fffffff));
+      unit[h][0] = __shfl_sync(0xffffffffu, u, 8 * tig);
+      unit[h][1] = __shfl_sync(0xffffffffu, u, 8 * tig + 4);
     }
   }
 
   float o[NH][kM][4];
-  float m[NH][2], l[NH][2];
+  // m: the heads' references; at = kLift - m. Before the first tile every power
+  // is infinite, which makes that tile set them.
+  float m[NH][2], at[NH][2], l[NH][2];
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
     m[h][0] = m[h][1] = -INFINITY;
+    at[h][0] = at[h][1] = 3.4028235e38f;
     l[h][0] = l[h][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < kM; ++i) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
@@ -245,112 +367,130 @@ __global__ void __launch_bounds__(kThreads) attn_paged_kernel(const __grid_const
   float vref = 0.f, inv_vref = 0.f;  // int8: power of two at or above the value scales met
   const float sl2 = a.scale_log2;
 
+  int st = 0, st_in = kStages - 1;  // stage of tile i, and of the tile issued beside it
   for (int i = 0; i < my_tiles; ++i) {
-    issue(i + kStages - 1, next_page);
+    issue(i + kStages - 1, next_page, st_in);
     next_page = page_of(i + kStages);
     cp_async_wait<kStages - 1>();
     __syncwarp();
     const int j0 = (tile0 + warp + i * kWarps) * kTile;
-    const unsigned char* sk = ring + (i % kStages) * R::kStageBytes;
+    const unsigned char* sk = ring + st * R::kStageBytes;
     const unsigned char* sv = sk + R::kTileBytes;
     const float* ss = reinterpret_cast<const float*>(sv + R::kTileBytes);
+    st_in = st;
+    st = st + 1 == kStages ? 0 : st + 1;
 
-    // S^T: two m16 tiles of positions x NH n8 tiles of heads
+    // S^T: two m16 tiles of positions x NH n8 tiles of heads; element e belongs
+    // to position gid + 8 (e >> 1), head 2 tig + (e & 1)
     float s[2][NH][4];
+    float f[2][2];  // what takes a position's scores to log2 units
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
+      if constexpr (!I8) {
 #pragma unroll
-      for (int h = 0; h < NH; ++h) s[mt][h][0] = s[mt][h][1] = s[mt][h][2] = s[mt][h][3] = 0.f;
-      if (!I8) {
+        for (int h = 0; h < NH; ++h) s[mt][h][0] = s[mt][h][1] = s[mt][h][2] = s[mt][h][3] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < kM; ++ks) {
+        for (int ks = 0; ks < kQ; ++ks) {
           uint32_t b[4];
           ldsm_x4(b, smem_u32(sk + swz<kRow>(mt * 16 + (lane & 15), 2 * ks + (lane >> 4))));
 #pragma unroll
-          for (int h = 0; h < NH; ++h) mma16816(s[mt][h], b[0], b[1], b[2], b[3], qb[h][ks][0], qb[h][ks][1]);
+          for (int h = 0; h < NH; ++h) mma16816(s[mt][h], b[0], b[1], b[2], b[3], qb[h][ks][0][0], qb[h][ks][1][0]);
         }
+        f[mt][0] = f[mt][1] = sl2;
       } else {
+        int c[NH][3][4] = {};
 #pragma unroll
-        for (int kp = 0; kp < kM / 2; ++kp) {
+        for (int ks = 0; ks < kQ; ++ks) {
           uint32_t b[4];
-          ldsm_x4(b, smem_u32(sk + swz<kRow>(mt * 16 + (lane & 15), 2 * kp + (lane >> 4))));
+          ldsm_x4(b, smem_u32(sk + swz<kRow>(mt * 16 + (lane & 15), 2 * ks + (lane >> 4))));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) b[e] ^= 0x80808080u;
+          for (int h = 0; h < NH; ++h) {
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t a0 = codes_h2<0x4140>(b[2 * e]), a2 = codes_h2<0x4342>(b[2 * e]);
-            const uint32_t a1 = codes_h2<0x4140>(b[2 * e + 1]), a3 = codes_h2<0x4342>(b[2 * e + 1]);
+            for (int d = 0; d < 3; ++d) mma16832(c[h][d], b, qb[h][ks][0][d], qb[h][ks][1][d]);
+          }
+        }
 #pragma unroll
-            for (int h = 0; h < NH; ++h) {
-              mma16816(s[mt][h], a0, a1, a2, a3, qb[h][2 * kp + e][0], qb[h][2 * kp + e][1]);
+        for (int h = 0; h < NH; ++h) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            // the first digit's sum stays below 2^21, the others' together below 2^28
+            const float low = static_cast<float>(c[h][1][e] * 128 + c[h][2][e]);
+            s[mt][h][e] = fmaf(static_cast<float>(c[h][0][e]), 0x1p14f, low) * unit[h][e & 1];
+          }
+        }
+        f[mt][0] = ss[mt * 16 + gid];
+        f[mt][1] = ss[mt * 16 + gid + 8];
+      }
+    }
+    float p[2][NH][4];
+    const bool last = j0 + kTile > n;
+    auto powers = [&]() {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) p[mt][h][e] = exp2_approx(fmaf(s[mt][h][e], f[mt][e >> 1], at[h][e & 1]));
+        }
+      }
+      if (last) {
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            if (j0 + mt * 16 + gid + 8 * (e >> 1) >= n) {
+#pragma unroll
+              for (int h = 0; h < NH; ++h) p[mt][h][e] = 0.f;
             }
           }
         }
       }
-      // log2 units; element e belongs to position gid + 8 (e >> 1), head 2 tig + (e & 1)
-      float f0 = sl2, f1 = sl2;
-      if (I8) {
-        f0 *= ss[mt * 16 + gid];
-        f1 *= ss[mt * 16 + gid + 8];
-      }
-#pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        s[mt][h][0] *= f0;
-        s[mt][h][1] *= f0;
-        s[mt][h][2] *= f1;
-        s[mt][h][3] *= f1;
-      }
-    }
-    if (j0 + kTile > n) {
-#pragma unroll
-      for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          if (j0 + mt * 16 + gid + 8 * (e >> 1) >= n) {
-#pragma unroll
-            for (int h = 0; h < NH; ++h) s[mt][h][e] = -INFINITY;
-          }
-        }
-      }
-    }
-    float top[NH][2];
-    bool over = false;
+    };
+    powers();
+    float most = 0.f;
 #pragma unroll
     for (int h = 0; h < NH; ++h) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        top[h][e] = fmaxf(fmaxf(s[0][h][e], s[0][h][e + 2]), fmaxf(s[1][h][e], s[1][h][e + 2]));
-        over |= top[h][e] > m[h][e] + kLag;
-      }
+      for (int e = 0; e < 4; ++e) most = fmaxf(most, fmaxf(p[0][h][e], p[1][h][e]));
     }
     float vs = 0.f;
+    bool over = most > kMost;
     if (I8) {
       vs = fabsf(ss[kTile + lane]);
       over |= vs > vref;
     }
     if (__any_sync(0xffffffffu, over)) {
-      float new_ref = vref, ratio = 1.f;
+      float ratio = 1.f;
       if (I8) {
         // the power of two above the largest scale of the tile (a NaN scale
         // never compares and poisons the probabilities by itself)
         const unsigned bits = __reduce_max_sync(0xffffffffu, vs <= 3.4028235e38f ? __float_as_uint(vs) : 0u);
         const float up = __uint_as_float(min((bits >> 23) + 1u, 0xfeu) << 23);
-        if (bits != 0u && up > vref) new_ref = up;
-        ratio = new_ref > 0.f ? vref / new_ref : 1.f;
-        vref = new_ref;
-        inv_vref = vref > 0.f ? 1.f / vref : 0.f;
+        if (bits != 0u && up > vref) {
+          ratio = vref / up;
+          vref = up;
+          inv_vref = 1.f / up;
+        }
       }
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
         float cr[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = fmaxf(top[h][e], m[h][e]);
+          float x = m[h][e];
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              if (j0 + mt * 16 + gid + 8 * half < n) x = fmaxf(x, s[mt][h][2 * half + e] * f[mt][half]);
+            }
+          }
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          cr[e] = m[h][e] == -INFINITY ? 0.f : exp2f(m[h][e] - x);
+          cr[e] = m[h][e] == -INFINITY ? 0.f : exp2_approx(m[h][e] - x);
           m[h][e] = x;
+          if (x != -INFINITY) at[h][e] = kLift - x;  // all scores -inf so far: still unset
           l[h][e] *= cr[e];
           cr[e] *= ratio;
         }
@@ -362,8 +502,9 @@ __global__ void __launch_bounds__(kThreads) attn_paged_kernel(const __grid_const
           o[h][k][3] *= cr[1];
         }
       }
+      powers();
     }
-    // probabilities, and P^T as B fragments: the transpose of each 8 x 8 block
+    // P^T as B fragments: the transpose of each 8 x 8 block
     uint32_t pb[2][NH][2];
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
@@ -374,15 +515,10 @@ __global__ void __launch_bounds__(kThreads) attn_paged_kernel(const __grid_const
       }
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
-        // a head whose every score so far is -inf keeps base 0
-        const float b0 = kLift - (m[h][0] == -INFINITY ? 0.f : m[h][0]);
-        const float b1 = kLift - (m[h][1] == -INFINITY ? 0.f : m[h][1]);
-        const float p0 = exp2f(s[mt][h][0] + b0), p1 = exp2f(s[mt][h][1] + b1);
-        const float p2 = exp2f(s[mt][h][2] + b0), p3 = exp2f(s[mt][h][3] + b1);
-        l[h][0] += p0 + p2;
-        l[h][1] += p1 + p3;
-        pb[mt][h][0] = transpose8x8(f2_to_h2(p0 * v0, p1 * v0));
-        pb[mt][h][1] = transpose8x8(f2_to_h2(p2 * v1, p3 * v1));
+        l[h][0] += p[mt][h][0] + p[mt][h][2];
+        l[h][1] += p[mt][h][1] + p[mt][h][3];
+        pb[mt][h][0] = transpose8x8(f2_to_h2(p[mt][h][0] * v0, p[mt][h][1] * v0));
+        pb[mt][h][1] = transpose8x8(f2_to_h2(p[mt][h][2] * v1, p[mt][h][3] * v1));
       }
     }
     // O^T += V^T P^T. fp16: m tile k holds dims 16 k + gid, + 8; int8: dims
@@ -390,25 +526,19 @@ __global__ void __launch_bounds__(kThreads) attn_paged_kernel(const __grid_const
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
       const int mtx = lane >> 3;
-      if (!I8) {
 #pragma unroll
-        for (int k = 0; k < kM; ++k) {
-          uint32_t b[4];
-          ldsm_x4_trans(b, smem_u32(sv + swz<kRow>(mt * 16 + 8 * (mtx >> 1) + (lane & 7), 2 * k + (mtx & 1))));
+      for (int kp = 0; kp < (I8 ? kM / 2 : kM); ++kp) {
+        uint32_t b[4];
+        if (!I8) {
+          ldsm_x4_trans(b, smem_u32(sv + swz<kRow>(mt * 16 + 8 * (mtx >> 1) + (lane & 7), 2 * kp + (mtx & 1))));
 #pragma unroll
-          for (int h = 0; h < NH; ++h) mma16816(o[h][k], b[0], b[1], b[2], b[3], pb[mt][h][0], pb[mt][h][1]);
-        }
-      } else {
-#pragma unroll
-        for (int kp = 0; kp < kM / 2; ++kp) {
-          uint32_t b[4];
+          for (int h = 0; h < NH; ++h) mma16816(o[h][kp], b[0], b[1], b[2], b[3], pb[mt][h][0], pb[mt][h][1]);
+        } else {
           ldsm_x4_trans(b, smem_u32(sv + swz<kRow>(mt * 16 + 8 * (mtx & 1) + (lane & 7), 2 * kp + (mtx >> 1))));
 #pragma unroll
-          for (int e = 0; e < 4; ++e) b[e] ^= 0x80808080u;
-#pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const uint32_t a0 = codes_h2<0x4240>(b[2 * e]), a1 = codes_h2<0x4341>(b[2 * e]);
-            const uint32_t a2 = codes_h2<0x4240>(b[2 * e + 1]), a3 = codes_h2<0x4341>(b[2 * e + 1]);
+            const uint32_t a0 = codes_h2(b[2 * e]), a1 = codes_h2(b[2 * e] >> 8);
+            const uint32_t a2 = codes_h2(b[2 * e + 1]), a3 = codes_h2(b[2 * e + 1] >> 8);
 #pragma unroll
             for (int h = 0; h < NH; ++h) mma16816(o[h][2 * kp + e], a0, a1, a2, a3, pb[mt][h][0], pb[mt][h][1]);
           }
@@ -430,10 +560,11 @@ __global__ void __launch_bounds__(kThreads) attn_paged_kernel(const __grid_const
   }
   __syncthreads();  // s_bad is initialised and every ring is idle: the rings hold the join
   if (__any_sync(0xffffffffu, bad) && lane == 0) s_bad = 1;
-  constexpr int kHeads = 8 * NH;
-  constexpr int kRedRow = D + 4;
-  float* red_o = reinterpret_cast<float*>(smem);          // [warps][heads][kRedRow]
-  float* red_ml = red_o + kWarps * kHeads * kRedRow;      // [warps][heads][2]
+  using J = Join<D, NH>;
+  float* red_o = reinterpret_cast<float*>(smem);
+  float* red_ml = red_o + kWarps * J::kHeads * J::kRedRow;
+  float* cta_o = red_ml + kWarps * J::kHeads * 2;  // [heads][D]
+  float* cta_ml = cta_o + J::kHeads * D;           // [heads][2], then the bad mark
   const float back = I8 ? vref : 1.f;
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
@@ -443,45 +574,89 @@ __global__ void __launch_bounds__(kThreads) attn_paged_kernel(const __grid_const
       for (int e = 0; e < 4; ++e) {
         const int head = h * 8 + 2 * tig + (e & 1);
         const int d = 16 * k + (I8 ? 2 * gid + (e >> 1) : gid + 8 * (e >> 1));
-        red_o[(warp * kHeads + head) * kRedRow + d] = o[h][k][e] * back;
+        red_o[(warp * J::kHeads + head) * J::kRedRow + d] = o[h][k][e] * back;
       }
     }
     if (gid == 0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        red_ml[(warp * kHeads + h * 8 + 2 * tig + e) * 2] = m[h][e];
-        red_ml[(warp * kHeads + h * 8 + 2 * tig + e) * 2 + 1] = l[h][e];
+        red_ml[(warp * J::kHeads + h * 8 + 2 * tig + e) * 2] = m[h][e];
+        red_ml[(warp * J::kHeads + h * 8 + 2 * tig + e) * 2 + 1] = l[h][e];
       }
     }
   }
   __syncthreads();
-  const bool any_bad = s_bad != 0;
+  bool any_bad = s_bad != 0;
   if (any_bad && threadIdx.x == 0 && g == 0) set_flag(a.err_flags, KLLM_B200_FLAG_BAD_PAGE);
-  const bool whole = per_part >= all_tiles;  // this part is all there is
+  // Head `head` of this cluster's positions: the output itself, or its share of it.
+  const bool whole = per_part * a.cluster >= all_tiles;
+  auto finish = [&](int head, int d, float acc, float top, float sum) {
+    if (whole) {
+      out_t[head * D + d] = __float2half_rn(any_bad ? 0.f : acc / sum);
+    } else {
+      const int64_t prow = (t * a.n_heads + static_cast<int64_t>(g) * G + head) * a.splits + cluster_part;
+      a.part_o[prow * D + d] = acc;
+      if (d == 0) {
+        a.part_ml[prow * 2] = top;
+        a.part_ml[prow * 2 + 1] = any_bad ? -1.f : sum;
+      }
+    }
+  };
   for (int idx = threadIdx.x; idx < G * D; idx += kThreads) {
     const int head = idx / D, d = idx - head * D;
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, red_ml[(w * kHeads + head) * 2]);
+    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, red_ml[(w * J::kHeads + head) * 2]);
     float L = 0.f, acc = 0.f;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       // a warp without tiles holds zeros and weight 0
-      const float f = join_weight(red_ml[(w * kHeads + head) * 2], M);
-      L += red_ml[(w * kHeads + head) * 2 + 1] * f;
-      acc += red_o[(w * kHeads + head) * kRedRow + d] * f;
+      const float x = join_weight(red_ml[(w * J::kHeads + head) * 2], M);
+      L += red_ml[(w * J::kHeads + head) * 2 + 1] * x;
+      acc += red_o[(w * J::kHeads + head) * J::kRedRow + d] * x;
     }
-    if (whole) {
-      out_t[idx] = __float2half_rn(any_bad ? 0.f : acc / L);
+    if (a.cluster == 1) {
+      finish(head, d, acc, M, L);
     } else {
-      const int64_t prow = (t * a.n_heads + static_cast<int64_t>(g) * G + head) * a.splits + part;
-      a.part_o[prow * D + d] = acc;
+      cta_o[idx] = acc;
       if (d == 0) {
-        a.part_ml[prow * 2] = M;
-        a.part_ml[prow * 2 + 1] = any_bad ? -1.f : L;
+        cta_ml[2 * head] = M;
+        cta_ml[2 * head + 1] = L;
       }
     }
   }
+  if (a.cluster == 1) return;
+  if (threadIdx.x == 0) cta_ml[2 * J::kHeads] = any_bad ? 1.f : 0.f;
+  cluster_sync();
+  const int rank = part - cluster_part * a.cluster;
+  for (int c = 0; c < a.cluster; ++c) any_bad |= ld_peer(cta_ml + 2 * J::kHeads, c) != 0.f;
+  for (int idx = rank * kThreads + threadIdx.x; idx < G * D; idx += a.cluster * kThreads) {
+    const int head = idx / D, d = idx - head * D;
+    float pm[kMaxCluster], pl[kMaxCluster], po[kMaxCluster];
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) {
+      if (c < a.cluster) {
+        pm[c] = ld_peer(cta_ml + 2 * head, c);
+        pl[c] = ld_peer(cta_ml + 2 * head + 1, c);
+        po[c] = ld_peer(cta_o + idx, c);
+      }
+    }
+    float M = -INFINITY, L = 0.f, acc = 0.f;
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) {
+      if (c < a.cluster) M = fmaxf(M, pm[c]);
+    }
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) {
+      if (c < a.cluster) {
+        const float x = join_weight(pm[c], M);
+        L += pl[c] * x;
+        acc += po[c] * x;
+      }
+    }
+    finish(head, d, acc, M, L);
+  }
+  cluster_sync();  // no CTA leaves while its shared memory may be read
 }
 
 // One warp per (token, query head) that has several parts.
@@ -498,42 +673,44 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attn_paged_combine_kernel(
   int flag;
   if (token_state(a.view, pos, seq, flag) != kTokenOk) return;
   const int all_tiles = (pos + kTile) / kTile;
-  const int per_part = (all_tiles + a.splits - 1) / a.splits;
-  const int used = (all_tiles + per_part - 1) / per_part;
+  const int parts = a.splits * a.cluster;
+  const int per_cluster = (all_tiles + parts - 1) / parts * a.cluster;
+  const int used = (all_tiles + per_cluster - 1) / per_cluster;
   if (used <= 1) return;
+  // lane c holds part c's max and sum; its weight goes to all by shuffles
   const float* ml = a.part_ml + row * a.splits * 2;
-  const float* po = a.part_o + row * a.splits * D;
-  float M = -INFINITY;
-  bool bad = false;
-  for (int c = lane; c < used; c += 32) {
-    M = fmaxf(M, ml[2 * c]);
-    bad |= ml[2 * c + 1] == -1.f;
+  const float* po = a.part_o + row * a.splits * D + lane * kPer;
+  float pm = -INFINITY, pl = 0.f;
+  if (lane < used) {
+    pm = ml[2 * lane];
+    pl = ml[2 * lane + 1];
   }
+  const bool bad = __any_sync(0xffffffffu, pl == -1.f);
+  float M = pm;
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
-  bad = __any_sync(0xffffffffu, bad);
-  float L = 0.f, acc[kPer];
+  const float weight = join_weight(pm, M);
+  const float L = group_sum<32>(weight * pl);
+  float acc[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
-  for (int c = 0; c < used; ++c) {
-    const float w = join_weight(ml[2 * c], M);
-    L += w * ml[2 * c + 1];
+  for (int c0 = 0; c0 < used; c0 += 8) {
+    float x[8][kPer];
 #pragma unroll
-    for (int k = 0; k < kPer; ++k) acc[k] += w * po[c * D + lane * kPer + k];
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) x[i][k] = c0 + i < used ? po[(c0 + i) * D + k] : 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float w = __shfl_sync(0xffffffffu, weight, c0 + i);
+#pragma unroll
+      for (int k = 0; k < kPer; ++k) acc[k] += w * x[i][k];
+    }
   }
   __half* dst = a.out + t * a.out_stride + (row - t * a.n_heads) * D + lane * kPer;
 #pragma unroll
   for (int k = 0; k < kPer; ++k) dst[k] = __float2half_rn(bad ? 0.f : acc[k] / L);
-}
-
-// Parts per (token, kv head): enough CTAs for several waves of the device.
-int64_t preferred_splits(int64_t items, int64_t capacity) {
-  const int64_t want = 8LL * sm_count();
-  int64_t s = (want + items - 1) / items;
-  const int64_t most = (capacity + kWarps * kTile - 1) / (kWarps * kTile);
-  if (s > most) s = most;
-  if (s > kMaxSplits) s = kMaxSplits;
-  return s < 1 ? 1 : s;
 }
 
 int64_t workspace_for(int64_t n_tokens, int64_t n_heads, int64_t head_dim, int64_t splits) {
@@ -549,20 +726,65 @@ int check_heads(const char* what, int64_t n_tokens, int64_t n_heads, int64_t hkv
   if (n_heads / hkv > kMaxGroups) {
     return fail(KLLM_B200_ERR_SHAPE, "%s: more than %d query heads per kv head", what, kMaxGroups);
   }
-  if (n_tokens * kMaxSplits > 0x7fffffffLL) return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
+  if (n_tokens * kMaxSplits * kMaxCluster > 0x7fffffffLL) return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
   return KLLM_B200_OK;
+}
+
+// How the positions of a (token, kv head) are dealt out, by sizes the host
+// knows: the largest cluster of which the device holds one for every item at
+// once, and, where the largest leaves room, several clusters per item while a
+// CTA's share of the capacity is at least 256 positions. A CTA costs about 6 us
+// of one slot beside its rows (positions, page table and first rows are read
+// one after another, and its parts are joined), so items that fill the device
+// by themselves are not split. Measured, us, clusters of 1 / 2 / 4 / 8 for
+// sequences of up to 4095 positions, 14 heads over 2 kv heads of 64:
+//   int8   8 sequences  23.4 / 16.2 / 10.9 /  9.4;   64: 27.8 / 20.8 / 17.9 / 22.8
+//   fp16 128 sequences  31.1 / 30.6 / 31.5 / 46.0;  512: 87.4 / 88.0 / 100  / 166
+struct Split {
+  int cluster, splits;
+};
+
+template <int D, bool I8, int NH>
+Split split_of(int64_t items, int64_t capacity) {
+  const void* kernel = reinterpret_cast<const void*>(attn_paged_kernel<D, I8, NH>);
+  const size_t smem = Ring<D, I8>::kBytes;
+  Split x = {1, 1};
+  (void)allow_smem(kernel, smem);  // occupancy is asked for with the opt-in in place
+  for (int c = kMaxCluster; c > 1; c /= 2) {
+    if (capacity < c * kWarps * kTile) continue;
+    const int fit = active_clusters_raw(kernel, kThreads, smem, c);
+    if (fit < items) continue;
+    x.cluster = c;
+    while (c == kMaxCluster && x.splits < kMaxSplits && items * x.splits * 2 <= fit &&
+           capacity >= int64_t{512} * c * x.splits) {
+      x.splits *= 2;
+    }
+    break;
+  }
+  return x;
+}
+
+Split preferred_split(int64_t items, int64_t capacity, int64_t head_dim, bool i8, int64_t groups) {
+  if (head_dim == 64) {
+    if (i8) return groups <= 8 ? split_of<64, true, 1>(items, capacity) : split_of<64, true, 2>(items, capacity);
+    return groups <= 8 ? split_of<64, false, 1>(items, capacity) : split_of<64, false, 2>(items, capacity);
+  }
+  if (i8) return groups <= 8 ? split_of<128, true, 1>(items, capacity) : split_of<128, true, 2>(items, capacity);
+  return groups <= 8 ? split_of<128, false, 1>(items, capacity) : split_of<128, false, 2>(items, capacity);
 }
 
 template <int D, bool I8, int NH>
 int launch_attention(const PagedAttnArgs& a, const LaunchOpts& o) {
   const char* what = "attention_paged";
   const size_t smem = Ring<D, I8>::kBytes;
-  static_assert(Ring<D, I8>::kBytes >= kWarps * 8 * NH * (D + 4 + 2) * 4, "the join fits the rings");
+  static_assert(Ring<D, I8>::kBytes >= Join<D, NH>::kBytes, "the join fits the rings");
   auto kernel = attn_paged_kernel<D, I8, NH>;
   cudaError_t err = allow_smem(reinterpret_cast<const void*>(kernel), smem);
   if (err != cudaSuccess) return launch_status(err, "attention_paged: shared memory opt-in");
-  const dim3 grid(static_cast<unsigned>(a.n_tokens * a.splits), static_cast<unsigned>(a.view.n_kv_heads));
-  const int rc = launch_status(launch(kernel, grid, dim3(kThreads), smem, o.stream, o.pdl, a), what);
+  const dim3 grid(static_cast<unsigned>(a.n_tokens * a.splits * a.cluster), static_cast<unsigned>(a.view.n_kv_heads));
+  err = a.cluster == 1 ? launch(kernel, grid, dim3(kThreads), smem, o.stream, o.pdl, a)
+                       : launch_clustered(kernel, grid, dim3(kThreads), smem, o.stream, o.pdl, a.cluster, a);
+  const int rc = launch_status(err, what);
   if (rc != KLLM_B200_OK || a.splits == 1) return rc;
   const int64_t rows = a.n_tokens * a.n_heads;
   const dim3 cgrid(static_cast<unsigned>((rows + kCombineWarps - 1) / kCombineWarps));
@@ -585,7 +807,9 @@ int attention_paged_workspace_bytes(int64_t n_tokens, int64_t n_heads, const kll
   int rc = paged_view(cache, what, &view);
   if (rc == KLLM_B200_OK) rc = check_heads(what, n_tokens, n_heads, view.n_kv_heads);
   if (rc != KLLM_B200_OK || n_tokens == 0) return rc;
-  *bytes = workspace_for(n_tokens, n_heads, cache->head_dim, preferred_splits(n_tokens * view.n_kv_heads, view.capacity));
+  const Split split = preferred_split(n_tokens * view.n_kv_heads, view.capacity, cache->head_dim,
+                                      cache->cache_dtype == KLLM_B200_I8, n_heads / view.n_kv_heads);
+  *bytes = workspace_for(n_tokens, n_heads, cache->head_dim, split.splits);
   return KLLM_B200_OK;
 }
 
@@ -610,8 +834,10 @@ int attention_paged(const void* q, int64_t q_stride, const kllm_b200_paged_cache
   if (workspace_bytes > 0 && (!workspace || !aligned16(workspace))) {
     return fail(KLLM_B200_ERR_ALIGN, "%s: workspace must be non-null and 16-byte aligned", what);
   }
-  int64_t splits = preferred_splits(n_tokens * a.view.n_kv_heads, a.view.capacity);
-  while (workspace_for(n_tokens, n_heads, D, splits) > (workspace ? workspace_bytes : 0)) splits = (splits + 1) / 2;
+  const Split split = preferred_split(n_tokens * a.view.n_kv_heads, a.view.capacity, D,
+                                      cache->cache_dtype == KLLM_B200_I8, n_heads / a.view.n_kv_heads);
+  int64_t splits = split.splits;
+  while (workspace_for(n_tokens, n_heads, D, splits) > (workspace ? workspace_bytes : 0)) splits /= 2;
   a.q = static_cast<const __half*>(q);
   a.q_stride = q_stride;
   a.out = static_cast<__half*>(out);
@@ -625,6 +851,7 @@ int attention_paged(const void* q, int64_t q_stride, const kllm_b200_paged_cache
   a.n_tokens = n_tokens;
   a.n_heads = static_cast<int>(n_heads);
   a.groups = static_cast<int>(n_heads / a.view.n_kv_heads);
+  a.cluster = split.cluster;
   a.splits = static_cast<int>(splits);
   a.err_flags = err_flags;
   a.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));

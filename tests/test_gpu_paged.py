@@ -515,6 +515,7 @@ def test_attention_workspace_and_strides(cuda, ops, dtype):
     packed = randh(rng, 2, (hq + 2 * hkv) * d).cuda()
     q = packed[:, :hq * d].unflatten(1, (hq, d))
     full = ops.attention_paged_workspace_bytes(2, hq, cache)
+    assert ops.attention_paged_workspace_bytes(2000, hq, cache) == 0  # a batch that fills the device needs none
     for nbytes in {0, 16, full // 3 // 16 * 16, full}:
         ws = torch.full((max(nbytes, 16) + 64,), 0x7f, dtype=torch.uint8, device="cuda")
         whole = torch.full((2, hq * d + 40), -5.0, dtype=torch.float16, device="cuda")

@@ -119,9 +119,7 @@ def test_attention_refusals(capi):
     assert size(4, 8, None, n) == capi.ERR_INVALID_ARG and n.value == 0
     assert size(4, 7, c, n) == capi.ERR_SHAPE
     assert size(0, 8, c, n) == capi.OK and n.value == 0
-    # a batch that fills the device needs no parts; a single long sequence does
-    assert size(100_000, 8, c, n) == capi.OK and n.value == 0
-    assert size(1, 8, cache(capi, max_pages=1 << 14), n) == capi.OK and n.value > 0
+    assert size(100_000, 8, c, n) == capi.OK and n.value == 0  # a batch that fills the device needs no parts
 
 
 def test_logprob_refusals(capi):
