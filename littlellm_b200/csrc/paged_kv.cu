@@ -69,6 +69,24 @@ __device__ __forceinline__ void load8(const void* p, int f32, int at, float (&f)
   }
 }
 
+// 1 / x to an ulp (normal x).
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+__device__ __forceinline__ unsigned long long f32x2_fma(unsigned long long a, unsigned long long b, unsigned long long c) {
+  unsigned long long r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ unsigned long long f32x2_add(unsigned long long a, unsigned long long b) {
+  unsigned long long r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
 // The larger of two values, NaN when either is.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -76,35 +94,65 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// rint(x / scale) as a code in the low byte. inv is 1 / scale rounded, so
-// x * inv is off by up to a step of fp32; one residual step (q += (x - q scale)
-// inv, as in division by a reciprocal) gives the quotient rounded, so a value
-// half way between two codes is seen as such and goes to the even one. Adding
-// 1.5 * 2^23 rounds to a whole number, ties to even.
-__device__ __forceinline__ uint32_t code_of(float x, float scale, float inv) {
-  const float q = x * inv;
-  return __float_as_uint(__fmaf_rn(__fmaf_rn(-q, scale, x), inv, q) + 12582912.f);
+// rint(x / scale) of 16 values as 16 codes. inv is 1 / scale to an ulp or two,
+// so q = x * inv is off by a few steps of fp32; one residual step
+// (q += (x - q scale) inv, as in division by a reciprocal) gives the quotient
+// rounded, so a value half way between two codes is seen as such and goes to
+// the even one. Adding 1.5 * 2^23 rounds to a whole number, ties to even, and
+// leaves the code in the low byte.
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], float scale, float inv) {
+  const unsigned long long i2 = f32x2_pack(inv, inv), n2 = f32x2_pack(-scale, -scale);
+  const unsigned long long magic = f32x2_pack(12582912.f, 12582912.f);
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    const unsigned long long v = f32x2_pack(x[i], x[i + 1]);
+    const unsigned long long q = f32x2_mul(v, i2);
+    const unsigned long long c = f32x2_add(f32x2_fma(f32x2_fma(q, n2, v), i2, q), magic);
+    float lo, hi;
+    f32x2_unpack(c, lo, hi);
+    w[i] = __float_as_uint(lo);
+    w[i + 1] = __float_as_uint(hi);
+  }
+  return make_uint2(__byte_perm(__byte_perm(w[0], w[1], 0x0040), __byte_perm(w[2], w[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(w[4], w[5], 0x0040), __byte_perm(w[6], w[7], 0x0040), 0x5410));
 }
 
-// Four codes packed into 32 bits.
-__device__ __forceinline__ uint32_t codes4(const float* x, float scale, float inv) {
-  const uint32_t lo = __byte_perm(code_of(x[0], scale, inv), code_of(x[1], scale, inv), 0x0040);
-  const uint32_t hi = __byte_perm(code_of(x[2], scale, inv), code_of(x[3], scale, inv), 0x0040);
-  return __byte_perm(lo, hi, 0x5410);
+// x *= r * w for eight values, two per packed multiply.
+__device__ __forceinline__ void scale8(float (&x)[8], float r, const float (&w)[8]) {
+  const unsigned long long r2 = f32x2_pack(r, r);
+#pragma unroll
+  for (int i = 0; i < 8; i += 2) {
+    f32x2_unpack(f32x2_mul(f32x2_pack(x[i], x[i + 1]), f32x2_mul(r2, f32x2_pack(w[i], w[i + 1]))), x[i], x[i + 1]);
+  }
 }
 
-template <int D, bool I8, int U>
-__global__ void __launch_bounds__(kThreads) qkv_norm_rope_append_paged_kernel(const __grid_constant__ AppendArgs a) {
+// Eight floats of shared memory (32-byte aligned).
+__device__ __forceinline__ void lds8(const float* p, float (&f)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  f[0] = a.x; f[1] = a.y; f[2] = a.z; f[3] = a.w; f[4] = b.x; f[5] = b.y; f[6] = b.z; f[7] = b.w;
+}
+
+// U sets of heads per warp. SHARED: every warp of the CTA works on the same
+// token, which computes its cos/sin once; else each warp computes its own
+// token's. Many tokens want warps more than registers: 16384 tokens of 96
+// heads of 128, int8, 148 us held to 9 CTAs per SM, 164 at the 7 that fit
+// unheld (103 us of HBM time; the rest is issue, about 290 instructions for
+// four heads, and the wait for the first loads of a warp).
+template <int D, bool I8, int U, bool SHARED>
+__global__ void __launch_bounds__(kThreads, SHARED && U > 1 ? (I8 ? 9 : 8) : 1) qkv_norm_rope_append_paged_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int L = D / 16;    // lanes of one head
   constexpr int kSet = 32 / L;  // heads a warp takes at once
-  __shared__ float2 s_cs[kWarps][D / 2];
+  constexpr int kTables = SHARED ? 1 : kWarps;
+  __shared__ __align__(32) float s_cos[kTables][D / 2], s_sin[kTables][D / 2], s_neg[kTables][D / 2];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t gw = static_cast<int64_t>(blockIdx.x) * kWarps + warp;
-  const int64_t t = gw / a.warps_per_token;
-  const int part = static_cast<int>(gw - t * a.warps_per_token);
+  // SHARED: CTA (x, y) takes part y of token x; else consecutive warps
+  const unsigned w0 = blockIdx.x * kWarps + warp, wpt = a.warps_per_token;
+  const int64_t t = SHARED ? blockIdx.x : w0 / wpt;
+  const int part = SHARED ? blockIdx.y * kWarps + warp : static_cast<int>(w0 - static_cast<unsigned>(t) * wpt);
   grid_dep_wait();
   grid_dep_launch();
-  if (t >= a.n_tokens) return;  // uniform per warp
+  if (t >= a.n_tokens) return;  // uniform per warp; with SHARED per CTA
 
   const int hkv = a.view.n_kv_heads;
   const int n_rows = a.n_heads + 2 * hkv;
@@ -135,20 +183,24 @@ __global__ void __launch_bounds__(kThreads) qkv_norm_rope_append_paged_kernel(co
     if (flag != 0 && part == 0 && lane == 0) set_flag(a.err_flags, flag);
     return;
   }
-#pragma unroll
-  for (int i = lane; i < D / 2; i += 32) {
+  const int table = SHARED ? 0 : warp;
+  for (int i = SHARED ? threadIdx.x : lane; i < D / 2; i += SHARED ? kThreads : 32) {
     const double w = static_cast<double>(pos) * a.turns[i];
     const float f = static_cast<float>(w - rint(w));
     float sn, cs;
     sincospif(2.f * f, &sn, &cs);
-    s_cs[warp][i] = make_float2(cs, sn);
+    s_cos[table][i] = cs;
+    s_sin[table][i] = sn;
+    s_neg[table][i] = -sn;
   }
-  __syncwarp();
+  if (SHARED) __syncthreads(); else __syncwarp();
   const int64_t row0 = ((static_cast<int64_t>(page) * hkv) << a.view.page_shift) + (pos & ((1 << a.view.page_shift) - 1));
 
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int h = (part * U + u) * kSet + lane / L;
+    const int h0 = (part * U + u) * kSet;  // the set's first head: what follows is uniform per warp where it can be
+    if (h0 >= n_rows) break;
+    const int h = h0 + lane / L;
     const bool live = h < n_rows, is_q = h < a.n_heads, is_v = h >= a.n_heads + hkv;
     const int hh = is_q ? h : is_v ? h - a.n_heads - hkv : h - a.n_heads;  // within its tensor
     float x[8], y[8], p[8];
@@ -163,34 +215,47 @@ __global__ void __launch_bounds__(kThreads) qkv_norm_rope_append_paged_kernel(co
 #pragma unroll
       for (int i = 0; i < 8; ++i) y[i] += p[i];
     }
-    float ss = 0.f;
+    if (h0 < a.n_heads + hkv) {  // some q or k head
+      if (a.q_norm != nullptr || a.k_norm != nullptr) {
+        unsigned long long s2 = 0ull;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], fmaf(y[i], y[i], ss));
+        for (int i = 0; i < 8; i += 2) {
+          const unsigned long long v = f32x2_pack(x[i], x[i + 1]), w = f32x2_pack(y[i], y[i + 1]);
+          s2 = f32x2_fma(v, v, f32x2_fma(w, w, s2));
+        }
+        float ss, s1;
+        f32x2_unpack(s2, ss, s1);
+        ss += s1;
 #pragma unroll
-    for (int m = L / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
-    const void* weight = is_v ? nullptr : is_q ? a.q_norm : a.k_norm;
-    if (live && weight != nullptr) {
-      const float r = rsqrtf(ss * (1.f / D) + a.eps);
-      load8(weight, a.norm_f32, 8 * c, p);
+        for (int m = L / 2; m > 0; m >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, m);
+        const void* weight = is_v ? nullptr : is_q ? a.q_norm : a.k_norm;
+        if (weight != nullptr) {
+          const float r = rsqrtf(ss * (1.f / D) + a.eps);
+          load8(weight, a.norm_f32, 8 * c, p);
+          scale8(x, r, p);
+          load8(weight, a.norm_f32, D / 2 + 8 * c, p);
+          scale8(y, r, p);
+        }
+      }
+      if (!is_v) {
+        float cs[8], sn[8], ns[8], rx[8], ry[8];
+        lds8(&s_cos[table][8 * c], cs);
+        lds8(&s_sin[table][8 * c], sn);
+        lds8(&s_neg[table][8 * c], ns);
+        rope_rotate8_x2(x, y, cs, sn, ns, rx, ry);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] *= r * p[i];
-      load8(weight, a.norm_f32, D / 2 + 8 * c, p);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] *= r * p[i];
-    }
-    if (!is_v) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 cs = s_cs[warp][8 * c + i];
-        const float x1 = x[i], x2 = y[i];
-        rope_rotate(x1, x2, cs.x, cs.y, x[i], y[i]);
+        for (int i = 0; i < 8; ++i) {
+          x[i] = rx[i];
+          y[i] = ry[i];
+        }
+      }
+      if (live && is_q) {
+        __half* dst = a.q_out + t * a.q_out_stride + hh * D + 8 * c;
+        st_plain(dst, pack8(x));
+        st_plain(dst + D / 2, pack8(y));
       }
     }
-    if (live && is_q) {
-      __half* dst = a.q_out + t * a.q_out_stride + hh * D + 8 * c;
-      st_plain(dst, pack8(x));
-      st_plain(dst + D / 2, pack8(y));
-    }
+    if (h0 + kSet <= a.n_heads) continue;  // no k or v head in the set
     const int64_t row = row0 + (static_cast<int64_t>(hh) << a.view.page_shift);
     if (!I8) {
       if (live && !is_q) {
@@ -208,27 +273,50 @@ __global__ void __launch_bounds__(kThreads) qkv_norm_rope_append_paged_kernel(co
         // below 2^-60 a row is zero in every use (fp16 ends at 2^-24) and its
         // reciprocal would leave fp32; an infinity or NaN marks the whole row
         const bool tiny = mx < 0x1p-60f, sound = mx <= 3.4028235e38f;
-        const float scale = tiny ? 0.f : mx / 127.f;
-        const float inv = tiny || !sound ? 0.f : 1.f / scale;
+        // mx / 127 rounded: a product and its residual step
+        const float s0 = mx * (1.f / 127.f), s1 = fmaf(fmaf(-127.f, s0, mx), 1.f / 127.f, s0);
+        const bool coded = sound && !tiny;
+        const float scale = coded ? s1 : 0.f, inv = coded ? rcp_approx(s1) : 0.f;
         if (!sound) {
 #pragma unroll
           for (int i = 0; i < 8; ++i) x[i] = y[i] = 0.f;
         }
         int8_t* dst = static_cast<int8_t*>(is_v ? a.v_pages : a.k_pages) + row * D + 8 * c;
-        const float step = sound ? scale : 0.f;
-        *reinterpret_cast<uint2*>(dst) = make_uint2(codes4(x, step, inv), codes4(x + 4, step, inv));
-        *reinterpret_cast<uint2*>(dst + D / 2) = make_uint2(codes4(y, step, inv), codes4(y + 4, step, inv));
+        *reinterpret_cast<uint2*>(dst) = codes8(x, scale, inv);
+        *reinterpret_cast<uint2*>(dst + D / 2) = codes8(y, scale, inv);
         if (c == 0) (is_v ? a.v_scales : a.k_scales)[row] = sound ? scale : __int_as_float(0x7fffffff);
       }
     }
   }
 }
 
+// How a token's sets of heads go to warps: u sets a warp, `warps` warps, whole
+// CTAs per token (shared) or not.
+struct Deal {
+  int u, warps;
+  bool shared;
+};
+
 template <int D, bool I8>
-void (*pick_append(int u))(AppendArgs) {
-  return u == 1 ? qkv_norm_rope_append_paged_kernel<D, I8, 1>
-         : u == 2 ? qkv_norm_rope_append_paged_kernel<D, I8, 2>
-                  : qkv_norm_rope_append_paged_kernel<D, I8, 3>;
+void (*pick_append(Deal d))(AppendArgs) {
+  if (!d.shared) return qkv_norm_rope_append_paged_kernel<D, I8, 3, false>;
+  return d.u == 1   ? qkv_norm_rope_append_paged_kernel<D, I8, 1, true>
+         : d.u == 2 ? qkv_norm_rope_append_paged_kernel<D, I8, 2, true>
+                    : qkv_norm_rope_append_paged_kernel<D, I8, 3, true>;
+}
+
+// Few tokens: one set a warp, which is the shortest path through a token. Many:
+// two or three sets a warp, which computes cos/sin for more heads at a time;
+// heads that do not fill a CTA then share one with other tokens. 14 + 2 * 2
+// heads of 64, int8, us (one set / three sets): 1 token 3.3 / 5.0, 1024 4.1 /
+// 5.5, 4096 9.6 / 10.8, 16384 33.7 / 29.9, 65536 123 / 98.9.
+Deal deal_sets(int64_t sets, int64_t n_tokens) {
+  auto warps = [&](int u) { return static_cast<int>((sets + u - 1) / u); };
+  auto whole = [&](int u) { return (warps(u) + kWarps - 1) / kWarps * kWarps; };  // in whole CTAs
+  if (n_tokens * whole(1) <= 16384) return {1, whole(1), true};
+  if (warps(3) < kWarps) return {3, warps(3), false};
+  const int u = 2 * whole(2) < 3 * whole(3) ? 2 : 3;  // the one that leaves fewer idle sets
+  return {u, whole(u), true};
 }
 
 // ---------------------------------------------------------------------------
@@ -250,23 +338,43 @@ struct ReadArgs {
   int64_t n_out_slots, out_max_seq;
   __half* k_out;
   __half* v_out;
+  bool wide;  // outputs 32-byte aligned
   int32_t* err_flags;
 };
 
-// Sixteen codes times the row's scale, as fp16.
+// Sixteen codes times the row's scale, as fp16. The byte c + 128 under the
+// exponent of 2^23 is the fp32 2^23 + c + 128; the difference is c exactly, the
+// product rounds to fp32 and then to fp16.
 __device__ __forceinline__ void dequant16(uint4 w, float scale, uint4& lo, uint4& hi) {
   const uint32_t r[4] = {w.x, w.y, w.z, w.w};
+  const unsigned long long s2 = f32x2_pack(scale, scale), off = f32x2_pack(-8388736.f, -8388736.f);
   uint32_t h[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int v = static_cast<int>(r[i]);
-    h[2 * i] = f2_to_h2(static_cast<float>(static_cast<int8_t>(v)) * scale,
-                        static_cast<float>(static_cast<int8_t>(v >> 8)) * scale);
-    h[2 * i + 1] = f2_to_h2(static_cast<float>(static_cast<int8_t>(v >> 16)) * scale,
-                            static_cast<float>(static_cast<int8_t>(v >> 24)) * scale);
+    const uint32_t b = r[i] ^ 0x80808080u;
+    const uint32_t e = 0x4b000000u;
+    const unsigned long long x =
+        f32x2_pack(__uint_as_float(__byte_perm(b, e, 0x7440)), __uint_as_float(__byte_perm(b, e, 0x7441)));
+    const unsigned long long y =
+        f32x2_pack(__uint_as_float(__byte_perm(b, e, 0x7442)), __uint_as_float(__byte_perm(b, e, 0x7443)));
+    float p, q;
+    f32x2_unpack(f32x2_mul(f32x2_add(x, off), s2), p, q);
+    h[2 * i] = f2_to_h2(p, q);
+    f32x2_unpack(f32x2_mul(f32x2_add(y, off), s2), p, q);
+    h[2 * i + 1] = f2_to_h2(p, q);
   }
   lo = make_uint4(h[0], h[1], h[2], h[3]);
   hi = make_uint4(h[4], h[5], h[6], h[7]);
+}
+
+// 32 bytes of an output row whose base is 16-byte aligned only.
+__device__ __forceinline__ void store32(__half* p, bool aligned, uint4 lo, uint4 hi) {
+  if (aligned) {
+    st_plain32(p, lo, hi);
+  } else {
+    st_plain(p, lo);
+    st_plain(p + 8, hi);
+  }
 }
 
 // A CTA reads one kv head of a block of consecutive tokens, so consecutive
@@ -329,13 +437,9 @@ __global__ void __launch_bounds__(kReadThreads) kv_read_paged_kernel(const __gri
     if (I8) {
       uint4 lo, hi;
       dequant16(kw[u], ks[u], lo, hi);
-      __half* d = a.k_out + dst[u] * D + 16 * c;
-      st_plain(d, lo);
-      st_plain(d + 8, hi);
+      store32(a.k_out + dst[u] * D + 16 * c, a.wide, lo, hi);
       dequant16(vw[u], vs[u], lo, hi);
-      d = a.v_out + dst[u] * D + 16 * c;
-      st_plain(d, lo);
-      st_plain(d + 8, hi);
+      store32(a.v_out + dst[u] * D + 16 * c, a.wide, lo, hi);
     } else {
       st_plain(a.k_out + dst[u] * D + 8 * c, kw[u]);
       st_plain(a.v_out + dst[u] * D + 8 * c, vw[u]);
@@ -461,15 +565,15 @@ int qkv_norm_rope_kv_append_paged(const void* q, int64_t q_stride, const void* k
   for (int d = 1; d < D / 2; ++d) a.turns[d] = a.turns[d - 1] * step;
   const int set = static_cast<int>(32 / (D / 16));
   const int64_t sets = (n_heads + 2 * hkv + set - 1) / set;
-  const int u = 3;
-  a.warps_per_token = static_cast<int>((sets + u - 1) / u);
-  const int64_t warps = n_tokens * a.warps_per_token;
-  if (warps > (int64_t{1} << 32)) return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
-  const unsigned grid = static_cast<unsigned>((warps + kWarps - 1) / kWarps);
+  const Deal deal = deal_sets(sets, n_tokens);
+  a.warps_per_token = deal.warps;
+  if (n_tokens * deal.warps >= (int64_t{1} << 31)) return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
+  const dim3 grid = deal.shared ? dim3(static_cast<unsigned>(n_tokens), static_cast<unsigned>(deal.warps / kWarps))
+                                : dim3(static_cast<unsigned>((n_tokens * deal.warps + kWarps - 1) / kWarps));
   const bool i8 = cache->cache_dtype == KLLM_B200_I8;
-  void (*kernel)(AppendArgs) = D == 64 ? (i8 ? pick_append<64, true>(u) : pick_append<64, false>(u))
-                                       : (i8 ? pick_append<128, true>(u) : pick_append<128, false>(u));
-  return launch_status(launch(kernel, dim3(grid), dim3(kThreads), 0, o.stream, o.pdl, a), what);
+  void (*kernel)(AppendArgs) = D == 64 ? (i8 ? pick_append<64, true>(deal) : pick_append<64, false>(deal))
+                                       : (i8 ? pick_append<128, true>(deal) : pick_append<128, false>(deal));
+  return launch_status(launch(kernel, grid, dim3(kThreads), 0, o.stream, o.pdl, a), what);
 }
 
 int kv_read_paged(const kllm_b200_paged_cache* cache, const int32_t* positions, const int32_t* seqs, int64_t n_tokens,
@@ -500,6 +604,7 @@ int kv_read_paged(const kllm_b200_paged_cache* cache, const int32_t* positions, 
   a.out_max_seq = out_max_seq;
   a.k_out = static_cast<__half*>(k_out);
   a.v_out = static_cast<__half*>(v_out);
+  a.wide = aligned32(k_out) && aligned32(v_out);
   a.err_flags = err_flags;
   if (cache->cache_dtype == KLLM_B200_I8) {
     return cache->head_dim == 64 ? launch_read<64, true, 1>(a, o) : launch_read<128, true, 1>(a, o);

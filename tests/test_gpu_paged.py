@@ -113,12 +113,17 @@ def test_append_strided_and_in_place(cuda, ops, dtype, packed, in_place):
     check_append(ops, rng, dtype, 4, 4, 128, 16, [7], [1], 2, bias=torch.float16, packed=packed, in_place=in_place)
 
 
-@pytest.mark.parametrize("hq,hkv,d", [(14, 2, 64), (32, 8, 128)])
-def test_append_many_tokens(cuda, ops, hq, hkv, d):
+@pytest.mark.parametrize("hq,hkv,d,n", [
+    (14, 2, 64, 301), (32, 8, 128, 301),
+    (14, 2, 64, 4100),    # tokens that share a CTA
+    (32, 8, 128, 1400),   # three sets of heads per warp
+    (40, 8, 128, 1100),   # two
+])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_append_many_tokens(cuda, ops, dtype, hq, hkv, d, n):
     """A decode batch: one token per sequence at scattered positions."""
     rng = np.random.default_rng(8)
-    n = 301
-    check_append(ops, rng, torch.int8, hq, hkv, d, 16, rng.integers(0, 50, n).tolist(), rng.permutation(n).tolist(),
+    check_append(ops, rng, dtype, hq, hkv, d, 16, rng.integers(0, 50, n).tolist(), rng.permutation(n).tolist(),
                  n, norm=torch.float16, bias=torch.float16, theta=1e6)
 
 
