@@ -13,14 +13,18 @@
 // log2 units: the rounding of c' moves all t alike and cancels. fp32 logits
 // subtract first (x log2 e would overflow at the type's end).
 //
-// Largest entries: every thread also keeps the maximum of what it read. The
-// k-th largest of these maxima bounds the row's k-th largest value from below,
-// and about k values reach it. The threads whose maximum does are listed, and
-// the CTA reads their values again together (from L2), listing those at or
-// above the bound. A list that overflows (many equal values) is replaced by an
-// exact scan with a sorted list per warp. Entries are ordered by (value, lower
-// id first) as one 64-bit number, so equal values have one order whatever the
-// schedule.
+// Largest entries: every thread also keeps the maximum of what it read, and the
+// CTA keeps values in shared memory: all of them where they fit (kKeep vectors),
+// else each thread's batch with its maximum. The k-th largest of 64 groups'
+// maxima bounds the row's k-th largest value from below, and little more than k
+// values reach it; they are listed from what was kept. Only where more of a
+// thread than its kept batch reaches the bound are its values read again, by the
+// whole CTA. (Reading them again in every case waits for HBM once more, behind
+// the streams of the other rows, since the rows under way do not stay in L2:
+// 2048 x 151936 fp16 with 5 / 20 entries took 115 / 139 us instead of KB_TIME.)
+// A list that overflows (many equal values) is replaced by an exact scan with a
+// sorted list per warp. Entries are ordered by (value, lower id first) as one
+// 64-bit number, so equal values have one order whatever the schedule.
 //
 // A row is read by a cluster of 1 to 8 CTAs whose parts are pushed to the
 // first one's shared memory: one launch, no workspace. Bound: rows * vocab
@@ -40,6 +44,7 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxTop = 32;
 constexpr int kMaxCluster = 8;
 constexpr int kListed = 512;   // values at or above the bound that fit
+constexpr int kKeep = 2560;    // vectors of a CTA that are all kept (40 KB)
 constexpr int kBatch = 4;      // 16-byte vectors a thread loads at once
 constexpr float kLag = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
@@ -124,13 +129,6 @@ struct Sums {
       }
       ref = to;
     }
-  }
-  __device__ __forceinline__ void join(Sums b) {
-    const float top = fmaxf(ref, b.ref);
-    rebase(top);
-    b.rebase(top);
-    s += b.s;
-    w += b.w;
   }
   // the reference in use: 0 while everything met is -inf
   __device__ __forceinline__ float base() const { return ref == -INFINITY ? 0.f : ref; }
@@ -274,41 +272,69 @@ struct Shared {
   int above[kWarps];
   float all_ref[kMaxCluster], all_s[kMaxCluster], all_w[kMaxCluster];  // first CTA: every CTA's sums
   int all_above[kMaxCluster];
-  int readers[kThreads];  // threads whose maximum reaches the bound
-  int n_readers;
+  uint32_t group[64];      // maxima of 64 groups of threads
+  int readers[kThreads];   // threads whose kept batch reaches the bound, from the front,
+  int reader_at[kThreads];  // its first vector; from the back, threads to read again
+  int n_readers, n_again;
   int n_listed;
   uint32_t bound;
 };
 
-// The part of a row one CTA reads: 16-byte vectors [v0, v1) of the aligned
-// body, and (first and last CTA) the single values before and after it.
+// The part of a row one CTA reads: n_vec 16-byte vectors of the aligned body,
+// and (first and last CTA) the single values before and after it.
 template <typename T>
 struct Part {
   const T* row;
   const uint4* body;
-  int64_t v0, v1;
-  int head, tail;       // single values before the body / after it that this CTA reads
-  int64_t body0, tail0;  // ids of the first body value and of the first tail value
+  int n_vec;
+  int head, tail;    // single values before the body / after it that this CTA reads
+  int body0, tail0;  // ids of the first value of this CTA's vectors and of the first tail value
 };
 
 template <typename T>
-__device__ __forceinline__ Part<T> part_of(const LogprobArgs& a, int64_t r, uint32_t rank, uint32_t n_cta) {
+__device__ __forceinline__ Part<T> part_of(const LogprobArgs& a, int64_t r, int rank, int cta_shift) {
   constexpr int N = Vec<T>::kN;
   Part<T> p;
   p.row = static_cast<const T*>(a.logits) + r * a.row_stride;
-  const int64_t lead =
-      static_cast<int64_t>(((16 - (reinterpret_cast<uintptr_t>(p.row) & 15)) & 15) / sizeof(T));
-  const int64_t head = lead < a.vocab ? lead : a.vocab;
-  const int64_t n_vec = (a.vocab - head) / N;
-  const int64_t per = (n_vec + n_cta - 1) / n_cta;
-  p.body = reinterpret_cast<const uint4*>(p.row + head);
-  p.v0 = min(per * rank, n_vec);
-  p.v1 = min(p.v0 + per, n_vec);
-  p.body0 = head;
+  const int vocab = static_cast<int>(a.vocab);  // <= 2^30
+  const int lead = static_cast<int>(((16 - (reinterpret_cast<uintptr_t>(p.row) & 15)) & 15) / sizeof(T));
+  const int head = min(lead, vocab);
+  const int n_vec = (vocab - head) / N;
+  const int per = (n_vec + (1 << cta_shift) - 1) >> cta_shift;
+  const int v0 = min(per * rank, n_vec);
+  p.n_vec = min(per, n_vec - v0);
+  p.body = reinterpret_cast<const uint4*>(p.row + head) + v0;
+  p.body0 = head + v0 * N;
   p.tail0 = head + n_vec * N;
-  p.head = rank == 0 ? static_cast<int>(head) : 0;
-  p.tail = rank == n_cta - 1 ? static_cast<int>(a.vocab - p.tail0) : 0;
+  p.head = rank == 0 ? head : 0;
+  p.tail = rank == (1 << cta_shift) - 1 ? vocab - p.tail0 : 0;
   return p;
+}
+
+// Joins the sums and counts of `n` (a power of two) lanes' worth of sets; every lane gets all.
+template <typename T>
+__device__ __forceinline__ void join_lanes(Sums<T>& a, int& count, int n) {
+  float top = a.ref;
+  for (int x = n / 2; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+  a.rebase(top);
+  for (int x = n / 2; x > 0; x >>= 1) {
+    a.s += __shfl_xor_sync(0xffffffffu, a.s, x);
+    a.w += __shfl_xor_sync(0xffffffffu, a.w, x);
+    count += __shfl_xor_sync(0xffffffffu, count, x);
+  }
+}
+
+// The 32 largest of two lists sorted over the lanes, largest first: of each
+// pair of opposite places the larger (a bitonic sequence), then its merge.
+__device__ __forceinline__ unsigned long long merge_lists(unsigned long long a, unsigned long long b, int lane) {
+  b = __shfl_sync(0xffffffffu, b, 31 - lane);
+  unsigned long long x = a > b ? a : b;
+#pragma unroll
+  for (int d = 16; d > 0; d >>= 1) {
+    const unsigned long long y = __shfl_xor_sync(0xffffffffu, x, d);
+    x = ((lane & d) != 0) == (x > y) ? y : x;
+  }
+  return x;
 }
 
 // Inserts the lanes' entries above the list's k-th into the warp's sorted list
@@ -327,13 +353,19 @@ __device__ __forceinline__ void insert_all(unsigned long long& list, unsigned lo
   }
 }
 
-template <typename T>
-__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __grid_constant__ LogprobArgs a, int n_cta) {
+template <typename T, bool KEEP_ALL>
+__global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __grid_constant__ LogprobArgs a,
+                                                                     int cta_shift) {
   constexpr int N = Vec<T>::kN;
+  // the CTA's vectors, or vector b of thread t's largest batch at b * kThreads + t
+  extern __shared__ uint4 kept_all[];
+  __shared__ uint4 kept_best[KEEP_ALL ? 1 : kBatch * kThreads];
+  uint4* const kept = KEEP_ALL ? kept_all : kept_best;
   __shared__ Shared sh;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t rank = n_cta > 1 ? cluster_rank() : 0;
-  const int64_t r = blockIdx.x / n_cta;
+  const int n_cta = 1 << cta_shift;
+  const int rank = n_cta > 1 ? static_cast<int>(cluster_rank()) : 0;
+  const int64_t r = blockIdx.x >> cta_shift;
   const int k = a.top_k;
   if (rank == 0) {
     for (int i = tid; i < n_cta * k; i += kThreads) sh.joined[i] = 0ull;
@@ -341,41 +373,59 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   if (n_cta > 1) cluster_arrive();  // waited for before the first store to a peer: by then it has cleared `joined`
   grid_dep_wait();
   grid_dep_launch();
-  const Part<T> p = part_of<T>(a, r, rank, n_cta);
-  const int n_vec = static_cast<int>(p.v1 - p.v0);  // of the CTA; vocab <= 2^30
-  const uint4* body = p.body + p.v0;
+  const int token = a.tokens != nullptr ? a.tokens[r] : -1;
+  const Part<T> p = part_of<T>(a, r, rank, cta_shift);
+  const int n_vec = p.n_vec;
   auto load = [&](Batch<T>& x, int at) {
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const int v = at + b * kThreads;
-      x.v[b] = v < n_vec ? __ldg(body + v) : Batch<T>::none();
+      x.v[b] = v < n_vec ? ld_stream(p.body + v) : Batch<T>::none();
     }
   };
   Batch<T> next;
   load(next, tid);
-  const int token = a.tokens != nullptr ? a.tokens[r] : -1;
   const bool asked = token >= 0 && token < a.vocab;
   const float given = asked ? to_f(p.row[token]) : INFINITY;
 
-  // ---- one read: sums, count above the given token, the thread's maximum
+  // ---- one read: sums, count above the given token, the thread's largest batch
   Sums<T> acc = {-INFINITY, 0.f, 0.f};
   int above = 0;
-  float most = -INFINITY;
+  int best_at = tid;  // first vector of the kept batch
+  float best = -INFINITY, second = -INFINITY, single = -INFINITY;
+  const float first = tid < p.head ? to_f(p.row[tid]) : -INFINITY;
+  const float last = tid < p.tail ? to_f(p.row[p.tail0 + tid]) : -INFINITY;
   auto take = [&](float x) {
-    most = fmaxf(most, x);
+    single = fmaxf(single, x);
     acc.admit(x);
     acc.add(x, acc.base());
     above += x > given;
   };
-  if (tid < p.head) take(to_f(p.row[tid]));
-  if (tid < p.tail) take(to_f(p.row[p.tail0 + tid]));
-  for (int at = tid; at < n_vec; at += kThreads * kBatch) {
+  if (tid < p.head) take(first);
+  if (tid < p.tail) take(last);
+  for (int at = tid; at - tid < n_vec; at += kThreads * kBatch) {
     const Batch<T> x = next;
     load(next, at + kThreads * kBatch);
     const float top = x.top();
-    most = fmaxf(most, top);
+    second = fmaxf(second, fminf(best, top));
     acc.admit(top);
     if (top > given) above += x.above(given);
+    if constexpr (KEEP_ALL) {
+      best = fmaxf(best, top);
+      if (k > 0) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) {
+          if (at + b * kThreads < n_vec) kept[at + b * kThreads] = x.v[b];
+        }
+      }
+    } else if (top > best) {
+      best = top;
+      if (k > 0) {
+#pragma unroll
+        for (int b = 0; b < kBatch; ++b) kept[b * kThreads + tid] = x.v[b];
+        best_at = at;
+      }
+    }
     unsigned long long s2 = f32x2_pack(acc.s, 0.f), w2 = f32x2_pack(acc.w, 0.f);
     x.add(acc.base(), s2, w2);
     float lo, hi;
@@ -386,98 +436,118 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   }
 
   // ---- the CTA's sums
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) {
-    Sums<T> b;
-    b.ref = __shfl_xor_sync(0xffffffffu, acc.ref, x);
-    b.s = __shfl_xor_sync(0xffffffffu, acc.s, x);
-    b.w = __shfl_xor_sync(0xffffffffu, acc.w, x);
-    acc.join(b);
-  }
-  above = __reduce_add_sync(0xffffffffu, above);
+  join_lanes(acc, above, 32);
   if (lane == 0) {
     sh.ref[warp] = acc.ref;
     sh.s[warp] = acc.s;
     sh.w[warp] = acc.w;
     sh.above[warp] = above;
   }
-  const uint32_t my_most = order_of(most);
-  sh.maxima[tid] = my_most;
-  if (tid == 0) sh.n_listed = sh.n_readers = 0;
+  sh.maxima[tid] = order_of(fmaxf(best, single));
+  if (tid == 0) sh.n_listed = sh.n_readers = sh.n_again = 0;
   if (n_cta > 1) cluster_wait();
   __syncthreads();
-  if (tid == kThreads - 1) {
-    Sums<T> all = {-INFINITY, 0.f, 0.f};
-    int n = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      all.join({sh.ref[w], sh.s[w], sh.w[w]});
-      n += sh.above[w];
-    }
-    if (rank == 0) {
-      sh.all_ref[0] = all.ref;
-      sh.all_s[0] = all.s;
-      sh.all_w[0] = all.w;
-      sh.all_above[0] = n;
-    } else {
-      push32(&sh.all_ref[rank], __float_as_uint(all.ref));
-      push32(&sh.all_s[rank], __float_as_uint(all.s));
-      push32(&sh.all_w[rank], __float_as_uint(all.w));
-      push32(&sh.all_above[rank], static_cast<uint32_t>(n));
+  if (warp == kWarps - 1) {
+    Sums<T> all = {sh.ref[lane % kWarps], sh.s[lane % kWarps], sh.w[lane % kWarps]};
+    int n = sh.above[lane % kWarps];
+    join_lanes(all, n, kWarps);
+    if (lane == 0) {
+      if (rank == 0) {
+        sh.all_ref[0] = all.ref;
+        sh.all_s[0] = all.s;
+        sh.all_w[0] = all.w;
+        sh.all_above[0] = n;
+      } else {
+        push32(&sh.all_ref[rank], __float_as_uint(all.ref));
+        push32(&sh.all_s[rank], __float_as_uint(all.s));
+        push32(&sh.all_w[rank], __float_as_uint(all.w));
+        push32(&sh.all_above[rank], static_cast<uint32_t>(n));
+      }
     }
   }
 
   if (k > 0) {
-    // ---- bound: the k-th largest of the threads' maxima, bit by bit from the
-    // first one in which they differ (fp16 values end at bit 13)
-    if (warp == 0) {
-      uint32_t mine[kThreads / 32], least = 0xffffffffu, largest = 0u;
+    // ---- bound: the k-th largest of 64 maxima, each over the same lane of
+    // every other warp, by the numbers above and at each; four lanes a group
+    const int g = tid >> 2, sub = tid & 3;
+    uint32_t mine = sh.maxima[(2 * sub + (g >> 5)) * 32 + (g & 31)];
+    mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 1));
+    mine = max(mine, __shfl_xor_sync(0xffffffffu, mine, 2));
+    if (sub == 0) sh.group[g] = mine;
+    __syncthreads();
+    int counts = 0;  // those above, and 2^16 times those at or above
 #pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) {
-        mine[i] = sh.maxima[i * 32 + lane];
-        least = min(least, mine[i]);
-        largest = max(largest, mine[i]);
-      }
-      least = __reduce_min_sync(0xffffffffu, least);
-      largest = __reduce_max_sync(0xffffffffu, largest);
-      constexpr int kLowBit = sizeof(T) == 2 ? 13 : 0;
-      const int first = 31 - __clz(least ^ largest);  // -1: all equal
-      uint32_t bound = first < 0 ? least : largest >> first >> 1 << first << 1;
-      for (int bit = first; bit >= kLowBit; --bit) {
-        const uint32_t trial = bound | (1u << bit);
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < kThreads / 32; ++i) n += mine[i] >= trial;
-        if (static_cast<int>(__reduce_add_sync(0xffffffffu, n)) >= k) bound = trial;
-      }
-      // threads without a value carry -inf as well: such a bound says nothing
-      if (lane == 0) sh.bound = bound <= kOrderNegInf ? 0u : bound;
+    for (int i = 0; i < 16; i += 4) {
+      const uint4 o = *reinterpret_cast<const uint4*>(&sh.group[16 * sub + i]);
+      counts += (o.x > mine) + (o.y > mine) + (o.z > mine) + (o.w > mine);
+      counts += ((o.x >= mine) + (o.y >= mine) + (o.z >= mine) + (o.w >= mine)) << 16;
     }
+    counts += __shfl_xor_sync(0xffffffffu, counts, 1);
+    counts += __shfl_xor_sync(0xffffffffu, counts, 2);
+    // threads without a value carry -inf as well: such a bound says nothing
+    if ((counts & 0xffff) < k && counts >> 16 >= k) sh.bound = mine <= kOrderNegInf ? 0u : mine;
     __syncthreads();
     const uint32_t bound = sh.bound;
-    if (my_most >= bound) sh.readers[atomicAdd(&sh.n_readers, 1)] = tid;
-    auto list_it = [&](float x, int64_t id) {
-      const uint32_t o = order_of(x);
-      if (o >= bound) {
-        const int at = atomicAdd(&sh.n_listed, 1);
-        if (at < kListed) sh.listed[at] = entry_of(o, static_cast<uint32_t>(id));
+    const float least = value_of(bound);  // NaN where everything counts
+    // the values of a vector that reach the bound
+    auto list_vector = [&](uint4 raw, int v) {
+      float x[N];
+      unpack(raw, x);
+      unsigned hits = 0u;
+#pragma unroll
+      for (int j = 0; j < N; ++j) hits |= x[j] >= least ? 1u << j : 0u;
+      if (bound == 0u) hits = (1u << N) - 1u;
+      if (hits != 0u) {
+        int at = atomicAdd(&sh.n_listed, __popc(hits));
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (hits >> j & 1u) {
+            if (at < kListed) sh.listed[at] = entry_of(order_of(x[j]), p.body0 + v * N + j);
+            ++at;
+          }
+        }
       }
     };
-    if (tid < p.head) list_it(to_f(p.row[tid]), tid);
-    if (tid < p.tail) list_it(to_f(p.row[p.tail0 + tid]), p.tail0 + tid);
+    auto list_single = [&](float x, int id) {
+      if (bound == 0u || x >= least) {
+        const int at = atomicAdd(&sh.n_listed, 1);
+        if (at < kListed) sh.listed[at] = entry_of(order_of(x), id);
+      }
+    };
+    if (tid < p.head) list_single(first, tid);
+    if (tid < p.tail) list_single(last, p.tail0 + tid);
+    if (!KEEP_ALL && (bound == 0u || second >= least)) {
+      sh.readers[kThreads - 1 - atomicAdd(&sh.n_again, 1)] = tid;
+    } else if (bound == 0u || best >= least) {
+      const int at = atomicAdd(&sh.n_readers, 1);
+      sh.readers[at] = tid;
+      sh.reader_at[at] = KEEP_ALL ? tid : best_at;
+    }
     __syncthreads();
-    const int n_readers = sh.n_readers;
-    for (int i = warp; i < n_readers; i += kWarps) {
-      const int from = sh.readers[i];
-      for (int v = from + lane * kThreads; v < n_vec; v += 32 * kThreads) {
-        float x[N];
-        unpack(__ldg(body + v), x);
-        float top = x[0];
+    // the kept vectors of the listed threads, dealt to all
+    const unsigned per_reader = (n_vec + kThreads - 1) / kThreads;  // vectors of a thread
+    const unsigned per_kept = KEEP_ALL ? per_reader : kBatch, n_kept = sh.n_readers * per_kept;
+    for (unsigned i = tid; i < n_kept; i += kThreads) {
+      if (*static_cast<volatile int*>(&sh.n_listed) > kListed) break;  // the list is full already
+      const unsigned q = i / per_kept, b = i - q * per_kept;
+      const int at = sh.reader_at[q] + b * kThreads;
+      if (at < n_vec) list_vector(kept[KEEP_ALL ? at : b * kThreads + sh.readers[q]], at);
+    }
+    // the vectors of the threads to read again
+    const unsigned n_items = sh.n_again * per_reader;
+    for (unsigned i0 = tid; i0 < n_items; i0 += kThreads * kBatch) {
+      if (*static_cast<volatile int*>(&sh.n_listed) > kListed) break;  // the list is full already
+      Batch<T> again;
+      int at[kBatch];
 #pragma unroll
-        for (int j = 1; j < N; ++j) top = fmaxf(top, x[j]);
-        if (bound == 0u || order_of(top) >= bound) {
+      for (int b = 0; b < kBatch; ++b) {
+        const unsigned i = i0 + b * kThreads, q = i / per_reader;
+        at[b] = i < n_items ? sh.readers[kThreads - 1 - q] + static_cast<int>(i - q * per_reader) * kThreads : n_vec;
+        again.v[b] = at[b] < n_vec ? __ldg(p.body + at[b]) : Batch<T>::none();
+      }
 #pragma unroll
-          for (int j = 0; j < N; ++j) list_it(x[j], p.body0 + (p.v0 + v) * N + j);
-        }
+      for (int b = 0; b < kBatch; ++b) {
+        if (at[b] < n_vec) list_vector(again.v[b], at[b]);
       }
     }
     __syncthreads();
@@ -485,20 +555,15 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
     if (n > kListed) {
       // ---- too many: a sorted list per warp over everything
       unsigned long long list = 0ull;
-      insert_all(list, tid < p.head ? entry_of(order_of(to_f(p.row[tid])), tid) : 0ull, k, lane);
-      insert_all(list,
-                 tid < p.tail ? entry_of(order_of(to_f(p.row[p.tail0 + tid])), static_cast<uint32_t>(p.tail0 + tid))
-                              : 0ull,
-                 k, lane);
+      insert_all(list, tid < p.head ? entry_of(order_of(first), tid) : 0ull, k, lane);
+      insert_all(list, tid < p.tail ? entry_of(order_of(last), p.tail0 + tid) : 0ull, k, lane);
       for (int v = warp * 32; v < n_vec; v += kThreads) {
         float x[N];
         const bool in = v + lane < n_vec;
-        unpack(in ? __ldg(body + v + lane) : make_uint4(0u, 0u, 0u, 0u), x);
+        unpack(in ? __ldg(p.body + v + lane) : make_uint4(0u, 0u, 0u, 0u), x);
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          insert_all(list,
-                     in ? entry_of(order_of(x[i]), static_cast<uint32_t>(p.body0 + (p.v0 + v + lane) * N + i)) : 0ull, k,
-                     lane);
+          insert_all(list, in ? entry_of(order_of(x[i]), p.body0 + (v + lane) * N + i) : 0ull, k, lane);
         }
       }
       __syncthreads();
@@ -506,12 +571,15 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
       n = kWarps * k;
       __syncthreads();
     }
-    // ---- the CTA's k largest: an entry's place is the number above it
-    for (int i = tid; i < n; i += kThreads) {
-      const unsigned long long e = sh.listed[i];
+    // ---- the CTA's k largest: an entry's place is the number above it, counted by eight lanes
+    for (int i0 = 0; i0 < n; i0 += kThreads / 8) {
+      const int i = i0 + tid / 8;
+      const unsigned long long e = i < n ? sh.listed[i] : 0ull;
       int place = 0;
-      for (int j = 0; j < n; ++j) place += sh.listed[j] > e;
-      if (place < k && e != 0ull) {
+      for (int j = tid % 8; j < n; j += 8) place += sh.listed[j] > e;
+#pragma unroll
+      for (int x = 1; x < 8; x <<= 1) place += __shfl_xor_sync(0xffffffffu, place, x);
+      if (tid % 8 == 0 && place < k && e != 0ull) {
         if (rank == 0) sh.joined[place] = e; else push64(&sh.joined[rank * k + place], e);
       }
     }
@@ -525,59 +593,72 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
     __syncthreads();
   }
   if (rank != 0) return;
-  Sums<T> all = {sh.all_ref[0], sh.all_s[0], sh.all_w[0]};
-  int count = sh.all_above[0];
-  for (int c = 1; c < n_cta; ++c) {
-    all.join({sh.all_ref[c], sh.all_s[c], sh.all_w[c]});
-    count += sh.all_above[c];
-  }
-  const bool nothing = all.s == 0.f;  // every logit is -inf
-  const float logs = log2f(all.s);
-  auto logprob = [&](float x) { return nothing ? -INFINITY : Scale<T>::log_of(x, all.ref, logs); };
-  if (tid == 0) {
-    if (a.tokens != nullptr) {
-      if (!asked && token != -1) set_flag(a.err_flags, KLLM_B200_FLAG_BAD_TOKEN);
-      a.logprobs[r] = asked ? logprob(given) : 0.f;
-      a.ranks[r] = asked ? 1 + count : 0;
+  if (warp == kWarps - 1) {
+    Sums<T> all = {sh.all_ref[lane % n_cta], sh.all_s[lane % n_cta], sh.all_w[lane % n_cta]};
+    int count = sh.all_above[lane % n_cta];
+    join_lanes(all, count, n_cta);
+    const bool nothing = all.s == 0.f;  // every logit is -inf
+    const float logs = nothing ? INFINITY : log2f(all.s);  // then every log probability is -inf
+    if (lane == 0) {
+      sh.ref[0] = nothing ? 0.f : all.ref;
+      sh.s[0] = logs;
+      if (a.tokens != nullptr) {
+        if (!asked && token != -1) set_flag(a.err_flags, KLLM_B200_FLAG_BAD_TOKEN);
+        a.logprobs[r] = !asked ? 0.f : nothing ? -INFINITY : Scale<T>::log_of(given, all.ref, logs);
+        a.ranks[r] = asked ? 1 + count : 0;
+      }
+      if (a.entropies != nullptr) {
+        const float h = (logs - all.w / all.s) * kLn2;
+        a.entropies[r] = nothing || h < 0.f ? 0.f : h;
+      }
     }
-    if (a.entropies != nullptr) {
-      const float h = (logs - all.w / all.s) * kLn2;
-      a.entropies[r] = nothing || h < 0.f ? 0.f : h;
-    }
   }
-  const int n = n_cta * k;  // <= kThreads
-  if (tid < n) {
+  if (k == 0) return;
+  // the cluster's lists, two by two
+  for (int m = n_cta / 2; m > 0; m /= 2) {
+    if (warp < m) {
+      const unsigned long long x = merge_lists(lane < k ? sh.joined[warp * k + lane] : 0ull,
+                                               lane < k ? sh.joined[(warp + m) * k + lane] : 0ull, lane);
+      if (lane < k) sh.joined[warp * k + lane] = x;
+    }
+    if (m > 1) __syncthreads();
+  }
+  __syncthreads();
+  if (tid < k) {
     const unsigned long long e = sh.joined[tid];
-    int place = tid;
-    if (n_cta > 1) {
-      place = 0;
-      for (int j = 0; j < n; ++j) place += sh.joined[j] > e;
-    }
-    if (place < k && e != 0ull) {
-      a.top_ids[r * k + place] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(e));
-      a.top_logprobs[r * k + place] = logprob(value_of(static_cast<uint32_t>(e >> 32)));
-    }
+    const float x = value_of(static_cast<uint32_t>(e >> 32));
+    a.top_ids[r * k + tid] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(e));
+    a.top_logprobs[r * k + tid] = sh.s[0] == INFINITY ? -INFINITY : Scale<T>::log_of(x, sh.ref[0], sh.s[0]);
   }
 }
 
-// CTAs per row: rows are split while the device has CTA slots to spare and a
-// CTA keeps at least 4096 values.
-int cluster_for(int64_t rows, int64_t vocab) {
-  int c = 1;
-  while (c < kMaxCluster && rows * c * 2 <= 2LL * sm_count() && vocab / (2 * c) >= 4096) c *= 2;
+// log2 of the CTAs per row: rows are split while the device has CTA slots to
+// spare and a CTA keeps at least 4096 values.
+int cluster_shift_for(int64_t rows, int64_t vocab) {
+  int c = 0;
+  while ((1 << c) < kMaxCluster && (rows << (c + 1)) <= 2LL * sm_count() && (vocab >> (c + 1)) >= 4096) ++c;
   return c;
 }
 
+template <typename T, bool KEEP_ALL>
+int launch_logprobs(const LogprobArgs& a, int cta_shift, int64_t kept, const LaunchOpts& o) {
+  auto kernel = token_logprobs_kernel<T, KEEP_ALL>;
+  cudaError_t err = allow_smem(reinterpret_cast<const void*>(kernel), kKeep * 16 + sizeof(Shared));
+  if (err != cudaSuccess) return launch_status(err, "token_logprobs: shared memory opt-in");
+  const size_t smem = a.top_k == 0 || !KEEP_ALL ? 0 : static_cast<size_t>(kept) * 16;
+  const dim3 grid(static_cast<unsigned>(a.rows << cta_shift));
+  err = cta_shift == 0 ? launch(kernel, grid, dim3(kThreads), smem, o.stream, o.pdl, a, 0)
+                       : launch_clustered(kernel, grid, dim3(kThreads), smem, o.stream, o.pdl, 1 << cta_shift, a,
+                                          cta_shift);
+  return launch_status(err, "token_logprobs");
+}
+
 template <typename T>
-int launch_logprobs(const LogprobArgs& a, const LaunchOpts& o) {
-  const char* what = "token_logprobs";
-  const int c = cluster_for(a.rows, a.vocab);
-  const dim3 grid(static_cast<unsigned>(a.rows * c));
-  if (c == 1) {
-    return launch_status(launch(token_logprobs_kernel<T>, grid, dim3(kThreads), 0, o.stream, o.pdl, a, c), what);
-  }
-  return launch_status(launch_clustered(token_logprobs_kernel<T>, grid, dim3(kThreads), 0, o.stream, o.pdl, c, a, c),
-                       what);
+int run_logprobs(const LogprobArgs& a, const LaunchOpts& o) {
+  const int c = cluster_shift_for(a.rows, a.vocab);
+  const int64_t vectors = ((a.vocab / Vec<T>::kN) >> c) + 1;  // of a CTA, at most
+  return vectors <= kKeep ? launch_logprobs<T, true>(a, c, vectors, o)
+                          : launch_logprobs<T, false>(a, c, kBatch * kThreads, o);
 }
 
 }  // namespace
@@ -607,7 +688,7 @@ int token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, i
   }
   LogprobArgs a = {logits,    rows,  vocab,   row_stride,   tokens,   logprobs, ranks,
                    entropies, top_k, top_ids, top_logprobs, err_flags};
-  return dtype == KLLM_B200_F16 ? launch_logprobs<__half>(a, o) : launch_logprobs<float>(a, o);
+  return dtype == KLLM_B200_F16 ? run_logprobs<__half>(a, o) : run_logprobs<float>(a, o);
 }
 
 }  // namespace kb
