@@ -31,6 +31,7 @@ FLAG_TIMEOUT = 16
 FLAG_BAD_SEQ = 32
 FLAG_BAD_PAGE = 64
 
+PAGED_SPLIT_MIN = 4096  # paged attention over a smaller capacity needs no workspace
 PARAM_IDS = 7680  # host ids carried per launch by kllm_b200_embedding_host_ids
 
 OP_EMBEDDING, OP_INPUT_NORM, OP_QKV_ROPE, OP_POST_NORM, OP_SWIGLU, OP_FINAL_NORM, OP_SELECT = (

@@ -733,7 +733,7 @@ int check_heads(const char* what, int64_t n_tokens, int64_t n_heads, int64_t hkv
 // How the positions of a (token, kv head) are dealt out, by sizes the host
 // knows: the largest cluster of which the device holds one for every item at
 // once, and, where the largest leaves room, several clusters per item while a
-// CTA's share of the capacity is at least 256 positions. A CTA costs about 6 us
+// CTA's share of the capacity stays at 256 positions or more. A CTA costs about 6 us
 // of one slot beside its rows (positions, page table and first rows are read
 // one after another, and its parts are joined), so items that fill the device
 // by themselves are not split. Measured, us, clusters of 1 / 2 / 4 / 8 for
@@ -756,7 +756,7 @@ Split split_of(int64_t items, int64_t capacity) {
     if (fit < items) continue;
     x.cluster = c;
     while (c == kMaxCluster && x.splits < kMaxSplits && items * x.splits * 2 <= fit &&
-           capacity >= int64_t{512} * c * x.splits) {
+           capacity >= int64_t{KLLM_B200_PAGED_SPLIT_MIN} * x.splits) {  // 512 positions of each of 8 CTAs
       x.splits *= 2;
     }
     break;

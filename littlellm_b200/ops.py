@@ -429,11 +429,14 @@ def dequantize_int8_batched(data: list[torch.Tensor], scales: list[torch.Tensor]
 def _call(device, entry, *args) -> None:
     """Calls a C entry point with `device` current (the context is entered only
     when it is not) and its stream appended, and checks the status."""
-    if device.index == torch.cuda.current_device():
-        check(entry(*args, _stream(device)))
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            check(entry(*args, _stream(device)))
+            status = entry(*args, _stream(device))
+    if status != _capi.OK:
+        check(status)
 
 
 def _all_on(device, *tensors) -> None:
@@ -533,16 +536,16 @@ def _token_index(x: torch.Tensor, n: int, what: str) -> None:
 
 def _parameters(expected, names: str, what: str) -> int:
     """Checks optional (tensor, number of values) pairs and returns their dtype's code."""
-    code = None
+    dtype = None
     for x, n in expected:
         if x is None:
             continue
         if x.numel() != n:
             raise KllmError(_capi.ERR_SHAPE, f"{what}: {names} must hold {n} values, got {x.numel()}")
-        if code is not None and code != dtype_code(x):
+        if dtype is not None and x.dtype != dtype:
             raise KllmError(_capi.ERR_DTYPE, f"{what}: {names} must share a dtype")
-        code = dtype_code(x)
-    return F16 if code is None else code
+        dtype = x.dtype
+    return F16 if dtype is None else _DTYPES.get(dtype, -1)  # -1: refused by the library
 
 
 def qkv_norm_rope_kv_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: PagedKVCache,
@@ -618,8 +621,11 @@ def kv_read_paged(cache: PagedKVCache, positions: torch.Tensor, seqs: torch.Tens
 
 def attention_paged_workspace_bytes(n_tokens: int, n_heads: int, cache: PagedKVCache) -> int:
     n = ctypes.c_int64(0)
-    with torch.cuda.device(cache.device):
+    if cache.device.index == torch._C._cuda_getDevice():
         check(lib.kllm_b200_attention_paged_workspace_bytes(n_tokens, n_heads, cache.descriptor(), n))
+    else:
+        with torch.cuda.device(cache.device):
+            check(lib.kllm_b200_attention_paged_workspace_bytes(n_tokens, n_heads, cache.descriptor(), n))
     return n.value
 
 
@@ -643,12 +649,13 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, positions: torch.Tenso
     _token_index(positions, T, what)
     _token_index(seqs, T, what)
     _all_on(dev, positions, seqs, workspace, err_flags)
-    if workspace is None:
+    nbytes = 0
+    if workspace is not None:
+        nbytes = workspace.numel() * workspace.element_size()
+    elif c.max_pages * c.page_size >= _capi.PAGED_SPLIT_MIN:
         nbytes = attention_paged_workspace_bytes(T, Hq, cache)
         if nbytes:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-    else:
-        nbytes = workspace.numel() * workspace.element_size()
     _call(dev, lib.kllm_b200_attention_paged, q.data_ptr(), sq, c, positions.data_ptr(), seqs.data_ptr(), T, Hq,
           out.data_ptr(), so, workspace.data_ptr() if nbytes else None, nbytes, _ptr(err_flags))
     return out
