@@ -226,6 +226,18 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
   grid_dep_wait();
   grid_dep_launch();
   const int pos = a.positions[t], seq = a.seqs[t];
+  const __half* q_t = a.q + t * a.q_stride + static_cast<int64_t>(g) * G * D;
+  // int8: four query values a thread and step, on their way while the page
+  // table is read
+  constexpr int kQuads = 8 * NH * D / 4 / kThreads;
+  uint2 raw[I8 ? kQuads : 1];
+  if constexpr (I8) {
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const int at = 4 * (threadIdx.x + i * kThreads);
+      raw[i] = at < G * D ? *reinterpret_cast<const uint2*>(q_t + at) : make_uint2(0u, 0u);
+    }
+  }
   __half* out_t = a.out + t * a.out_stride + static_cast<int64_t>(g) * G * D;
   int flag;
   if (token_state(a.view, pos, seq, flag) != kTokenOk) {  // alike in every CTA of the cluster
@@ -305,50 +317,58 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
   int next_page = page_of(kStages - 1);
 
   // B fragments of Q^T: fp16 pairs, or (int8) the three digits of four dims
-  // each, with what takes a head's integer sums back to its scale.
+  // each, with what takes a head's integer sums back to its scale. The digits
+  // are made once per CTA (each warp for itself took 2 to 3 us of a CTA's life).
   constexpr int kQ = I8 ? D / 32 : kM;  // k steps of K Q^T
   uint32_t qb[NH][kQ][2][I8 ? 3 : 1];
   float unit[NH][2];
+  if constexpr (!I8) {
 #pragma unroll
-  for (int h = 0; h < NH; ++h) {
-    const int head = h * 8 + gid;
-    const bool live = head < G;
-    const __half* qh = a.q + t * a.q_stride + (static_cast<int64_t>(g) * G + (live ? head : 0)) * D;
-    if constexpr (!I8) {
-#pragma unroll
-      for (int ks = 0; ks < kQ; ++ks) {
-        qb[h][ks][0][0] = live ? *reinterpret_cast<const uint32_t*>(qh + ks * 16 + 2 * tig) : 0u;
-        qb[h][ks][1][0] = live ? *reinterpret_cast<const uint32_t*>(qh + ks * 16 + 2 * tig + 8) : 0u;
-      }
-    } else {
-      uint2 raw[kQ][2];
-      float qmax = 0.f;
+    for (int h = 0; h < NH; ++h) {
+      const int head = h * 8 + gid;
+      const __half* qh = q_t + (head < G ? head : 0) * D;
 #pragma unroll
       for (int ks = 0; ks < kQ; ++ks) {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          raw[ks][e] = live ? *reinterpret_cast<const uint2*>(qh + ks * 32 + 16 * e + 4 * tig) : make_uint2(0u, 0u);
-          const float2 x = h2_to_f2(raw[ks][e].x), y = h2_to_f2(raw[ks][e].y);
-          qmax = max_nan(qmax, max_nan(max_nan(fabsf(x.x), fabsf(x.y)), max_nan(fabsf(y.x), fabsf(y.y))));
-        }
+        qb[h][ks][0][0] = head < G ? *reinterpret_cast<const uint32_t*>(qh + ks * 16 + 2 * tig) : 0u;
+        qb[h][ks][1][0] = head < G ? *reinterpret_cast<const uint32_t*>(qh + ks * 16 + 2 * tig + 8) : 0u;
       }
-      qmax = max_nan(qmax, __shfl_xor_sync(0xffffffffu, qmax, 1));
-      qmax = max_nan(qmax, __shfl_xor_sync(0xffffffffu, qmax, 2));
+    }
+  } else {
+    __shared__ uint32_t s_digits[3][8 * NH * D / 4];
+    __shared__ float s_unit[8 * NH];
+#pragma unroll
+    for (int i = 0; i < kQuads; ++i) {
+      const int quad = threadIdx.x + i * kThreads;  // D / 4 lanes of a warp hold a head
+      const float2 x = h2_to_f2(raw[i].x), y = h2_to_f2(raw[i].y);
+      float qmax = max_nan(max_nan(fabsf(x.x), fabsf(x.y)), max_nan(fabsf(y.x), fabsf(y.y)));
+#pragma unroll
+      for (int d = D / 8; d > 0; d >>= 1) qmax = max_nan(qmax, __shfl_xor_sync(0xffffffffu, qmax, d));
       const float inv = qmax > 0.f ? 2080768.f / qmax : 0.f;  // 127 * 2^14
+      const float v[4] = {x.x * inv, x.y * inv, y.x * inv, y.y * inv};
+      uint32_t w[3];
+      digits(v, w);
+#pragma unroll
+      for (int d = 0; d < 3; ++d) s_digits[d][quad] = w[d];
+      // an infinite or NaN query makes the unit, and with it every score, NaN
+      if (quad % (D / 4) == 0) {
+        s_unit[quad / (D / 4)] =
+            qmax * (a.scale_log2 / 2080768.f) * (qmax <= 65504.f ? 1.f : __int_as_float(0x7fffffff));
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int h = 0; h < NH; ++h) {
 #pragma unroll
       for (int ks = 0; ks < kQ; ++ks) {
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float2 x = h2_to_f2(raw[ks][e].x), y = h2_to_f2(raw[ks][e].y);
-          const float v[4] = {x.x * inv, x.y * inv, y.x * inv, y.y * inv};
-          digits(v, qb[h][ks][e]);
+#pragma unroll
+          for (int d = 0; d < 3; ++d) qb[h][ks][e][d] = s_digits[d][(h * 8 + gid) * (D / 4) + ks * 8 + 4 * e + tig];
         }
       }
-      // the heads of this lane's scores are 2 tig and 2 tig + 1; an infinite or
-      // NaN query makes the unit, and with it every score, NaN
-      const float u = qmax * (a.scale_log2 / 2080768.f) * (qmax <= 65504.f ? 1.f : __int_as_float(0x7fffffff));
-      unit[h][0] = __shfl_sync(0xffffffffu, u, 8 * tig);
-      unit[h][1] = __shfl_sync(0xffffffffu, u, 8 * tig + 4);
+      // the heads of this lane's scores are 2 tig and 2 tig + 1
+      unit[h][0] = s_unit[h * 8 + 2 * tig];
+      unit[h][1] = s_unit[h * 8 + 2 * tig + 1];
     }
   }
 
