@@ -116,6 +116,22 @@ __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
+// The same with c = a * b (no registers to clear first).
+__device__ __forceinline__ void mma16816_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};\n"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma16832_new(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+      "{%10,%10,%10,%10};\n"
+      : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+}
 __device__ __forceinline__ void mma16832(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -266,9 +282,9 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
     const int j = (tile0 + warp + i * kWarps) * kTile + lane;
     return i < my_tiles && j < n ? __ldg(table + (j >> shift)) : -1;
   };
-  const char* const k_bytes = static_cast<const char*>(a.k_pages);
-  const char* const v_bytes = static_cast<const char*>(a.v_pages);
   const int lane_row = lane / kChunks, lane_ch = lane % kChunks;
+  const char* const k_bytes = static_cast<const char*>(a.k_pages) + lane_row * kRow + lane_ch * 16;
+  const char* const v_bytes = static_cast<const char*>(a.v_pages) + lane_row * kRow + lane_ch * 16;
   // Copies warp tile i into stage `st`; rows past the last position are
   // zero-filled, so no stale bits reach the products.
   auto issue = [&](int i, int page, int st) {
@@ -289,20 +305,21 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
         cp_async4(smem_u32(ss + kTile + lane), a.v_scales + row, ok ? 4 : 0);
       }
       const int64_t row_bytes = row * kRow;
+      auto copy = [&](bool all) {
 #pragma unroll
-      for (int o = 0; o < kTile / 8; ++o) {
-        // rows 8 o .. 8 o + 7 follow one another in one page (page 0's first rows where there are none)
-        const int64_t off = __shfl_sync(0xffffffffu, row_bytes, 8 * o) + lane_row * kRow + lane_ch * 16;
-        const char* kp = k_bytes + off;
-        const char* vp = v_bytes + off;
+        for (int o = 0; o < kTile / 8; ++o) {
+          // rows 8 o .. 8 o + 7 follow one another in one page (page 0's first rows where there are none)
+          const int64_t off = __shfl_sync(0xffffffffu, row_bytes, 8 * o);
 #pragma unroll
-        for (int it = 0; it < 8 / kStep; ++it) {
-          const int r = 8 * o + it * kStep + lane_row;
-          const int bytes = (live >> r) & 1 ? 16 : 0;
-          cp_async16(smem_u32(sk + swz<kRow>(r, lane_ch)), kp + it * kStep * kRow, bytes);
-          cp_async16(smem_u32(sv + swz<kRow>(r, lane_ch)), vp + it * kStep * kRow, bytes);
+          for (int it = 0; it < 8 / kStep; ++it) {
+            const int r = 8 * o + it * kStep + lane_row;
+            const int bytes = all || (live >> r) & 1 ? 16 : 0;
+            cp_async16(smem_u32(sk + swz<kRow>(r, lane_ch)), k_bytes + off + it * kStep * kRow, bytes);
+            cp_async16(smem_u32(sv + swz<kRow>(r, lane_ch)), v_bytes + off + it * kStep * kRow, bytes);
+          }
         }
-      }
+      };
+      if (live == 0xffffffffu) copy(true); else copy(false);
     }
     cp_async_commit();  // empty groups keep the count uniform
   };
@@ -408,17 +425,18 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
     for (int mt = 0; mt < 2; ++mt) {
       if constexpr (!I8) {
 #pragma unroll
-        for (int h = 0; h < NH; ++h) s[mt][h][0] = s[mt][h][1] = s[mt][h][2] = s[mt][h][3] = 0.f;
-#pragma unroll
         for (int ks = 0; ks < kQ; ++ks) {
           uint32_t b[4];
           ldsm_x4(b, smem_u32(sk + swz<kRow>(mt * 16 + (lane & 15), 2 * ks + (lane >> 4))));
 #pragma unroll
-          for (int h = 0; h < NH; ++h) mma16816(s[mt][h], b[0], b[1], b[2], b[3], qb[h][ks][0][0], qb[h][ks][1][0]);
+          for (int h = 0; h < NH; ++h) {
+            if (ks == 0) mma16816_new(s[mt][h], b[0], b[1], b[2], b[3], qb[h][ks][0][0], qb[h][ks][1][0]);
+            else mma16816(s[mt][h], b[0], b[1], b[2], b[3], qb[h][ks][0][0], qb[h][ks][1][0]);
+          }
         }
         f[mt][0] = f[mt][1] = sl2;
       } else {
-        int c[NH][3][4] = {};
+        int c[NH][3][4];
 #pragma unroll
         for (int ks = 0; ks < kQ; ++ks) {
           uint32_t b[4];
@@ -426,7 +444,10 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
 #pragma unroll
           for (int h = 0; h < NH; ++h) {
 #pragma unroll
-            for (int d = 0; d < 3; ++d) mma16832(c[h][d], b, qb[h][ks][0][d], qb[h][ks][1][d]);
+            for (int d = 0; d < 3; ++d) {
+              if (ks == 0) mma16832_new(c[h][d], b, qb[h][ks][0][d], qb[h][ks][1][d]);
+              else mma16832(c[h][d], b, qb[h][ks][0][d], qb[h][ks][1][d]);
+            }
           }
         }
 #pragma unroll
