@@ -49,7 +49,7 @@ int resident_ctas(Kernel kernel, int threads, size_t smem) {
 int active_clusters_raw(const void* kernel, int threads, size_t smem, int cluster);
 
 // Opt `kernel` in to `smem` bytes of dynamic shared memory when that exceeds
-// the 48 KB default (once per kernel and size).
+// the 48 KB default (once per kernel, size and device).
 cudaError_t allow_smem(const void* kernel, size_t smem);
 
 // Grid for a grid-stride kernel: one full wave of resident CTAs, never more

@@ -65,8 +65,9 @@ int g_occ_n = 0;
 struct SmemEntry {
   const void* kernel;
   size_t smem;
+  int device;  // the opt-in belongs to a device's context
 };
-SmemEntry g_smem[64];
+SmemEntry g_smem[512];
 int g_smem_n = 0;
 }  // namespace
 
@@ -116,13 +117,15 @@ int active_clusters_raw(const void* kernel, int threads, size_t smem, int cluste
 
 cudaError_t allow_smem(const void* kernel, size_t smem) {
   if (smem <= 48 * 1024) return cudaSuccess;
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
   std::lock_guard<std::mutex> lock(g_occ_mutex);
   for (int i = 0; i < g_smem_n; ++i) {
-    if (g_smem[i].kernel == kernel && g_smem[i].smem >= smem) return cudaSuccess;
+    if (g_smem[i].kernel == kernel && g_smem[i].device == device && g_smem[i].smem >= smem) return cudaSuccess;
   }
-  const cudaError_t err =
-      cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-  if (err == cudaSuccess && g_smem_n < 64) g_smem[g_smem_n++] = {kernel, smem};
+  err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+  if (err == cudaSuccess && g_smem_n < 512) g_smem[g_smem_n++] = {kernel, smem, device};
   return err;
 }
 
