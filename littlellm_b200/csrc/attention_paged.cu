@@ -700,24 +700,30 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
   cluster_sync();  // no CTA leaves while its shared memory may be read
 }
 
-// One warp per (token, query head) that has several parts.
+// One warp per (token, query head) that has several parts. Always launched with
+// programmatic dependent launch: positions and sequences are read before the
+// wait (the attention kernel lets dependents start only after its own wait, so
+// whatever wrote them is done), the parts after it, all at once.
 template <int D>
 __global__ void __launch_bounds__(kCombineWarps * 32) attn_paged_combine_kernel(const __grid_constant__ PagedAttnArgs a) {
   constexpr int kPer = D / 32;
   const int lane = threadIdx.x & 31;
   const int64_t row = static_cast<int64_t>(blockIdx.x) * kCombineWarps + (threadIdx.x >> 5);
+  int used = 0;
+  if (row < a.n_tokens * a.n_heads) {
+    const int64_t t = row / a.n_heads;
+    const int pos = a.positions[t], seq = a.seqs[t];
+    int flag;
+    if (token_state(a.view, pos, seq, flag) == kTokenOk) {
+      const int all_tiles = (pos + kTile) / kTile;
+      const int parts = a.splits * a.cluster;
+      const int per_cluster = (all_tiles + parts - 1) / parts * a.cluster;
+      used = (all_tiles + per_cluster - 1) / per_cluster;
+    }
+  }
   grid_dep_wait();
   grid_dep_launch();
-  if (row >= a.n_tokens * a.n_heads) return;
-  const int64_t t = row / a.n_heads;
-  const int pos = a.positions[t], seq = a.seqs[t];
-  int flag;
-  if (token_state(a.view, pos, seq, flag) != kTokenOk) return;
-  const int all_tiles = (pos + kTile) / kTile;
-  const int parts = a.splits * a.cluster;
-  const int per_cluster = (all_tiles + parts - 1) / parts * a.cluster;
-  const int used = (all_tiles + per_cluster - 1) / per_cluster;
-  if (used <= 1) return;
+  if (used <= 1) return;  // written by the attention kernel
   // lane c holds part c's max and sum; its weight goes to all by shuffles
   const float* ml = a.part_ml + row * a.splits * 2;
   const float* po = a.part_o + row * a.splits * D + lane * kPer;
@@ -726,29 +732,28 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attn_paged_combine_kernel(
     pm = ml[2 * lane];
     pl = ml[2 * lane + 1];
   }
+  float x[kMaxSplits][kPer];
+#pragma unroll
+  for (int c = 0; c < kMaxSplits; ++c) {
+#pragma unroll
+    for (int k = 0; k < kPer; ++k) x[c][k] = c < used ? po[c * D + k] : 0.f;
+  }
   const bool bad = __any_sync(0xffffffffu, pl == -1.f);
   float M = pm;
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, x));
+  for (int i = 16; i > 0; i >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, i));
   const float weight = join_weight(pm, M);
   const float L = group_sum<32>(weight * pl);
   float acc[kPer];
 #pragma unroll
   for (int k = 0; k < kPer; ++k) acc[k] = 0.f;
-  for (int c0 = 0; c0 < used; c0 += 8) {
-    float x[8][kPer];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
+  for (int c = 0; c < kMaxSplits; ++c) {
+    const float w = __shfl_sync(0xffffffffu, weight, c);
 #pragma unroll
-      for (int k = 0; k < kPer; ++k) x[i][k] = c0 + i < used ? po[(c0 + i) * D + k] : 0.f;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float w = __shfl_sync(0xffffffffu, weight, c0 + i);
-#pragma unroll
-      for (int k = 0; k < kPer; ++k) acc[k] += w * x[i][k];
-    }
+    for (int k = 0; k < kPer; ++k) acc[k] += w * x[c][k];
   }
+  const int64_t t = row / a.n_heads;
   __half* dst = a.out + t * a.out_stride + (row - t * a.n_heads) * D + lane * kPer;
 #pragma unroll
   for (int k = 0; k < kPer; ++k) dst[k] = __float2half_rn(bad ? 0.f : acc[k] / L);

@@ -513,25 +513,31 @@ def _head_rows(x: torch.Tensor, heads: int | None, head_dim: int, device, what: 
     """Checks x [n_tokens, heads, head_dim] on `device`, fp16 with contiguous
     heads, and returns the elements between its tokens (views into one packed
     projection pass)."""
-    if x.get_device() != device.index:
-        raise KllmError(_capi.ERR_INVALID_ARG,
-                        "tensors are on different devices" if x.is_cuda else "expected a CUDA tensor")
-    if x.dtype != torch.float16:
-        raise KllmError(_capi.ERR_DTYPE, f"{what}: q, k, v and outputs must be float16")
-    shape = x.shape
-    if len(shape) != 3 or shape[2] != head_dim or (heads is not None and shape[1] != heads):
-        raise KllmError(_capi.ERR_SHAPE, f"{what}: expected [n_tokens, heads, {head_dim}], got {tuple(shape)}")
-    token, head, element = x.stride()
-    if element != 1 or (head != head_dim and shape[1] > 1):
+    shape, stride = x.shape, x.stride()
+    if (x.dtype is not torch.float16 or x.get_device() != device.index or len(shape) != 3 or shape[2] != head_dim
+            or (heads is not None and shape[1] != heads) or stride[2] != 1
+            or (stride[1] != head_dim and shape[1] > 1)):
+        if x.get_device() != device.index:
+            raise KllmError(_capi.ERR_INVALID_ARG,
+                            "tensors are on different devices" if x.is_cuda else "expected a CUDA tensor")
+        if x.dtype != torch.float16:
+            raise KllmError(_capi.ERR_DTYPE, f"{what}: q, k, v and outputs must be float16")
+        if len(shape) != 3 or shape[2] != head_dim or (heads is not None and shape[1] != heads):
+            raise KllmError(_capi.ERR_SHAPE, f"{what}: expected [n_tokens, heads, {head_dim}], got {tuple(shape)}")
         raise KllmError(_capi.ERR_SHAPE, f"{what}: the heads of a token must be contiguous")
-    return token if shape[0] > 1 else shape[1] * head_dim  # the stride of a single token is never used
+    return stride[0] if shape[0] > 1 else shape[1] * head_dim  # the stride of a single token is never used
 
 
-def _token_index(x: torch.Tensor, n: int, what: str) -> None:
-    if x.dtype != torch.int32:
-        raise KllmError(_capi.ERR_DTYPE, f"{what}: positions, seqs and slots must be int32")
-    if x.shape != (n,):
-        raise KllmError(_capi.ERR_SHAPE, f"{what}: positions, seqs and slots must be [n_tokens]")
+def _token_index(n: int, device, what: str, *tensors) -> None:
+    """Checks positions, seqs, slots or tokens: int32 [n] on `device`, contiguous."""
+    for x in tensors:
+        if x is not None and (x.dtype is not torch.int32 or x.dim() != 1 or x.shape[0] != n
+                              or x.get_device() != device.index or not x.is_contiguous()):
+            if x.dtype != torch.int32:
+                raise KllmError(_capi.ERR_DTYPE, f"{what}: positions, seqs, slots and tokens must be int32")
+            if x.shape != (n,):
+                raise KllmError(_capi.ERR_SHAPE, f"{what}: positions, seqs, slots and tokens must hold one entry each")
+            _all_on(device, x)
 
 
 def _parameters(expected, names: str, what: str) -> int:
@@ -571,11 +577,13 @@ def qkv_norm_rope_kv_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     sk, sv = _head_rows(k, Hkv, D, dev, what), _head_rows(v, Hkv, D, dev, what)
     if not (k.shape[0] == v.shape[0] == q_out.shape[0] == T):
         raise KllmError(_capi.ERR_SHAPE, f"{what}: q, k, v and q_out must hold the same number of tokens")
-    _token_index(positions, T, what)
-    _token_index(seqs, T, what)
-    _all_on(dev, positions, seqs, bq, bk, bv, q_norm, k_norm, err_flags)
-    bias = _parameters(((bq, Hq * D), (bk, Hkv * D), (bv, Hkv * D)), "biases", what)
-    norm = _parameters(((q_norm, D), (k_norm, D)), "norm weights", what)
+    _token_index(T, dev, what, positions, seqs)
+    _all_on(dev, bq, bk, bv, q_norm, k_norm, err_flags)
+    bias = norm = F16
+    if bq is not None or bk is not None or bv is not None:
+        bias = _parameters(((bq, Hq * D), (bk, Hkv * D), (bv, Hkv * D)), "biases", what)
+    if q_norm is not None or k_norm is not None:
+        norm = _parameters(((q_norm, D), (k_norm, D)), "norm weights", what)
     _call(dev, lib.kllm_b200_qkv_norm_rope_kv_append_paged, q.data_ptr(), sq, k.data_ptr(), sk, v.data_ptr(), sv,
           _ptr(bq), _ptr(bk), _ptr(bv), bias, _ptr(q_norm), _ptr(k_norm), norm, eps, theta, positions.data_ptr(),
           seqs.data_ptr(), T, Hq, c, q_out.data_ptr(), so, _ptr(err_flags))
@@ -594,8 +602,7 @@ def kv_read_paged(cache: PagedKVCache, positions: torch.Tensor, seqs: torch.Tens
     what = "kv_read_paged"
     c, dev = cache.descriptor(), cache.device
     T = positions.numel()
-    _token_index(positions, T, what)
-    _token_index(seqs, T, what)
+    _token_index(T, dev, what, positions, seqs, out_slots)
     if out_slots is None:
         shape, n_slots, max_seq = (T, c.n_kv_heads, c.head_dim), 0, 0
         if k_out is None:
@@ -603,7 +610,6 @@ def kv_read_paged(cache: PagedKVCache, positions: torch.Tensor, seqs: torch.Tens
         if v_out is None:
             v_out = torch.zeros(shape, dtype=torch.float16, device=dev)
     else:
-        _token_index(out_slots, T, what)
         if k_out is None or v_out is None or k_out.dim() != 4:
             raise KllmError(_capi.ERR_SHAPE, f"{what}: out_slots needs k_out and v_out [n_slots, kv_heads, max_seq, "
                                              "head_dim]")
@@ -613,7 +619,7 @@ def kv_read_paged(cache: PagedKVCache, positions: torch.Tensor, seqs: torch.Tens
         raise KllmError(_capi.ERR_SHAPE, f"{what}: outputs must be {shape}")
     if k_out.dtype != torch.float16 or v_out.dtype != torch.float16:
         raise KllmError(_capi.ERR_DTYPE, f"{what}: outputs must be float16")
-    _all_on(dev, positions, seqs, out_slots, k_out, v_out, err_flags)
+    _all_on(dev, k_out, v_out, err_flags)
     _call(dev, lib.kllm_b200_kv_read_paged, c, positions.data_ptr(), seqs.data_ptr(), T, _ptr(out_slots), n_slots,
           max_seq, k_out.data_ptr(), v_out.data_ptr(), _ptr(err_flags))
     return k_out, v_out
@@ -646,9 +652,8 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, positions: torch.Tenso
     so = _head_rows(out, Hq, D, dev, what)
     if out.shape[0] != T:
         raise KllmError(_capi.ERR_SHAPE, f"{what}: q and out must hold the same number of tokens")
-    _token_index(positions, T, what)
-    _token_index(seqs, T, what)
-    _all_on(dev, positions, seqs, workspace, err_flags)
+    _token_index(T, dev, what, positions, seqs)
+    _all_on(dev, workspace, err_flags)
     nbytes = 0
     if workspace is not None:
         nbytes = workspace.numel() * workspace.element_size()
@@ -703,10 +708,10 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
         out = token_logprobs_buffers(logits, top_k, tokens is not None)
     logprobs, ranks, entropies, top_ids, top_logprobs = out
     if tokens is not None:
-        _token_index(tokens, rows, what)
+        _token_index(rows, dev, what, tokens)
         if logprobs is None or ranks is None:
             raise KllmError(_capi.ERR_INVALID_ARG, f"{what}: tokens need logprobs and ranks among the outputs")
-    _all_on(dev, tokens, logprobs, ranks, entropies, top_ids, top_logprobs, err_flags)
+    _all_on(dev, logprobs, ranks, entropies, top_ids, top_logprobs, err_flags)
     for t, kind, shape in ((logprobs, torch.float32, (rows,)), (ranks, torch.int32, (rows,)),
                            (entropies, torch.float32, (rows,)), (top_ids, torch.int32, (rows, top_k)),
                            (top_logprobs, torch.float32, (rows, top_k))):
