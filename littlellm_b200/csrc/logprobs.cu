@@ -21,7 +21,7 @@
 // thread than its kept batch reaches the bound are its values read again, by the
 // whole CTA. (Reading them again in every case waits for HBM once more, behind
 // the streams of the other rows, since the rows under way do not stay in L2:
-// 2048 x 151936 fp16 with 5 / 20 entries took 115 / 139 us instead of KB_TIME.)
+// 2048 x 151936 fp16 with 5 / 20 entries took 120 / 137 us instead of 116 / 119.)
 // A list that overflows (many equal values) is replaced by an exact scan with a
 // sorted list per warp. Entries are ordered by (value, lower id first) as one
 // 64-bit number, so equal values have one order whatever the schedule.

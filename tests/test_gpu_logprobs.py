@@ -93,7 +93,7 @@ def tokens_for(rng, rows, vocab):
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
 @pytest.mark.parametrize("rows,vocab,k", [
     (1, 151936, 20), (3, 32000, 5), (1, 1, 1), (2, 2, 2), (5, 7, 7), (4, 31, 8), (9, 256, 32), (3, 2047, 32),
-    (2, 8193, 1), (17, 4099, 0), (700, 1000, 3), (150, 32003, 20),
+    (2, 8193, 1), (17, 4099, 0), (700, 1000, 3), (150, 32003, 20), (1, 1000003, 32), (400, 50021, 32),
 ])
 def test_against_float64(cuda, ops, dtype, rows, vocab, k):
     rng = np.random.default_rng(rows * 7 + vocab)

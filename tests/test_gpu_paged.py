@@ -565,6 +565,162 @@ def test_attention_bad_tokens_are_zero_and_flagged(cuda, ops):
         assert int(err.item()) == flag, (p, s)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_infinite_and_nan_queries(cuda, ops, dtype):
+    """A head whose query holds an infinity or NaN becomes NaN; the other heads
+    of its group, computed in the same tiles, do not."""
+    rng = np.random.default_rng(41)
+    hq, hkv, d, page = 8, 2, 64, 16
+    table, n_pages = pu.page_table(rng, [100, 100], page)
+    cache, k, v = pu.random_cache(rng, ops, dtype, n_pages, hkv, page, d, table)
+    q = randh(rng, 2, hq, d)
+    bad = q.clone()
+    bad[0, 1, 3] = float("nan")
+    bad[1, 6, 63] = float("inf")
+    bad[1, 6, 0] = 1.0
+    out = ops.attention_paged(bad.cuda(), cache, i32([99, 99]), i32([0, 1])).cpu()
+    assert torch.isnan(out[0, 1]).all() and torch.isnan(out[1, 6]).all()
+    for t, skip in ((0, 1), (1, 6)):
+        want, bound = pu.attention(q[t].double(), pu.rows_of(k, table, t, 100), pu.rows_of(v, table, t, 100))
+        for h in set(range(hq)) - {skip}:
+            assert ((out[t, h].double() - want[h]).abs() <= bound[h]).all()
+
+
+def test_attention_extreme_codes(cuda, ops):
+    """Every code a byte can hold, -128 among them, and queries at the ends of fp16."""
+    rng = np.random.default_rng(42)
+    hq, hkv, d, page, n = 4, 2, 64, 8, 64
+    table, n_pages = pu.page_table(rng, [n], page)
+    cache, k, v = pu.random_cache(rng, ops, torch.int8, n_pages, hkv, page, d, table)
+    codes = torch.from_numpy(rng.integers(-128, 128, k.shape, dtype=np.int8))
+    cache.k_pages.copy_(codes)
+    cache.v_pages.copy_(codes.flip(-1))
+    cache.k_scales.fill_(1e-7)
+    cache.v_scales.fill_(0.5)
+    k, v = codes.double() * float(cache.k_scales[0, 0, 0]), codes.flip(-1).double() * 0.5
+    q = torch.from_numpy(rng.choice([65504.0, -65504.0, 6e-8, 0.0, 1.0], (1, hq, d))).half()
+    out = ops.attention_paged(q.cuda(), cache, i32([n - 1]), i32([0])).cpu().double()
+    want, bound = pu.attention(q[0].double(), pu.rows_of(k, table, 0, n), pu.rows_of(v, table, 0, n))
+    assert ((out[0] - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("pdl", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_attention_split_in_a_graph(cuda, ops, dtype, pdl):
+    """A long cache whose parts go through the workspace, captured once and
+    replayed at positions that fill all parts, some, one, and none; the
+    positions are written by a kernel of the same graph."""
+    rng = np.random.default_rng(43)
+    hq, hkv, d, page, n = 4, 1, 64, 64, 20000
+    table, n_pages = pu.page_table(rng, [n], page)
+    cache, k, v = pu.random_cache(rng, ops, dtype, n_pages, hkv, page, d, table)
+    q = randh(rng, 1, hq, d, scale=2.0).cuda()
+    nbytes = ops.attention_paged_workspace_bytes(1, hq, cache)
+    assert nbytes > 0
+    ws = torch.full((nbytes,), 0xff, dtype=torch.uint8, device="cuda")  # NaN everywhere
+    given, positions, seqs = i32([5]), i32([-1]), i32([0])
+    out = torch.empty(1, hq, d, dtype=torch.float16, device="cuda")
+    previous = ops.set_pdl(pdl)
+    try:
+        def step():
+            torch.add(given, 0, out=positions)
+            ops.attention_paged(q, cache, positions, seqs, out=out, workspace=ws)
+
+        step()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+    finally:
+        ops.set_pdl(previous)
+    for pos in (n - 1, 12345, 300, 0, -1, 31, n - 1):
+        given.fill_(pos)
+        graph.replay()
+        torch.cuda.synchronize()
+        if pos < 0:
+            assert bool((out == 0).all())
+        else:
+            want, bound = pu.attention(q[0].cpu().double(), pu.rows_of(k, table, 0, pos + 1),
+                                       pu.rows_of(v, table, 0, pos + 1))
+            assert ((out[0].cpu().double() - want).abs() <= bound).all(), pos
+
+
+def test_attention_two_streams_at_once(cuda, ops):
+    """Calls that overlap on two streams, each with the workspace its call makes."""
+    rng = np.random.default_rng(44)
+    hq, hkv, d, page, n = 4, 1, 64, 64, 20000
+    table, n_pages = pu.page_table(rng, [n, n], page)
+    cache, _, _ = pu.random_cache(rng, ops, torch.float16, n_pages, hkv, page, d, table)
+    q = [randh(rng, 1, hq, d).cuda() for _ in range(2)]
+    at = [(i32([n - 1 - i]), i32([i])) for i in range(2)]
+    want = [ops.attention_paged(q[i], cache, *at[i]).clone() for i in range(2)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for _ in range(30):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, ops.attention_paged(q[i], cache, *at[i])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want[i]) for i, x in got)
+
+
+def test_no_tokens(cuda, ops):
+    cache = ops.PagedKVCache.allocate(2, 16, 2, 64, 1, 2, dtype=torch.int8)
+    none, q, kv = i32([]), torch.empty(0, 4, 64, dtype=torch.float16, device="cuda"), None
+    kv = torch.empty(0, 2, 64, dtype=torch.float16, device="cuda")
+    assert ops.qkv_norm_rope_kv_append_paged(q, kv, kv, cache, none, none, 1e4).shape == q.shape
+    assert ops.attention_paged(q, cache, none, none).shape == q.shape
+    assert all(x.shape == (0, 2, 64) for x in ops.kv_read_paged(cache, none, none))
+    assert ops.token_logprobs(torch.empty(0, 50, dtype=torch.float16, device="cuda"), none, 3).top_ids.shape == (0, 3)
+    torch.cuda.synchronize()
+
+
+def test_wrapper_refusals(cuda, ops):
+    """Shapes, dtypes and layouts that the C entry points cannot see."""
+    from littlellm_b200 import _capi
+    cache = ops.PagedKVCache.allocate(2, 16, 2, 64, 1, 2)
+    q, kv, at = (torch.zeros(3, 4, 64, dtype=torch.float16, device="cuda"),
+                 torch.zeros(3, 2, 64, dtype=torch.float16, device="cuda"), i32([0, 1, 2]))
+    codes = torch.zeros(2, 2, 16, 64, dtype=torch.int8, device="cuda")
+    scales = torch.zeros(2, 2, 16, device="cuda")
+    calls = [
+        (_capi.ERR_DTYPE, lambda: ops.attention_paged(q.float(), cache, at, at)),
+        (_capi.ERR_DTYPE, lambda: ops.attention_paged(q, cache, at.long(), at)),
+        (_capi.ERR_SHAPE, lambda: ops.attention_paged(q, cache, at[:2], at)),
+        (_capi.ERR_SHAPE, lambda: ops.attention_paged(q[:, :3], cache, at, at)),          # 3 heads over 2
+        (_capi.ERR_SHAPE, lambda: ops.attention_paged(q.transpose(0, 1), cache, at, at)),
+        (_capi.ERR_SHAPE, lambda: ops.attention_paged(q.expand(3, 4, 64)[..., :32], cache, at, at)),
+        (_capi.ERR_SHAPE, lambda: ops.attention_paged(q[:1].expand(3, 4, 64), cache, at, at)),  # one row for all tokens
+        (_capi.ERR_SHAPE, lambda: ops.attention_paged(q, cache, at, at, out=q[:2])),
+        (_capi.ERR_SHAPE, lambda: ops.qkv_norm_rope_kv_append_paged(q, kv[:2], kv, cache, at, at, 1e4)),
+        (_capi.ERR_SHAPE, lambda: ops.qkv_norm_rope_kv_append_paged(q, kv, kv, cache, at, at, 1e4, q_norm=q[0, 0, :32])),
+        (_capi.ERR_SHAPE, lambda: ops.qkv_norm_rope_kv_append_paged(q, kv, kv, cache, at, at, 1e4, bq=q[0, 0])),
+        (_capi.ERR_DTYPE, lambda: ops.qkv_norm_rope_kv_append_paged(q, kv, kv, cache, at, at, 1e4, q_norm=q[0, 0].int(),
+                                                                    k_norm=q[0, 0].int())),
+        (_capi.ERR_DTYPE, lambda: ops.qkv_norm_rope_kv_append_paged(q, kv, kv, cache, at, at, 1e4, q_norm=q[0, 0],
+                                                                    k_norm=q[0, 0].float())),
+        (_capi.ERR_INVALID_ARG, lambda: ops.attention_paged(q, cache, at.cpu(), at)),
+        (_capi.ERR_SHAPE, lambda: ops.kv_read_paged(cache, at, at, out_slots=at)),
+        (_capi.ERR_SHAPE, lambda: ops.kv_read_paged(cache, at, at, k_out=kv[:2], v_out=kv)),
+        (_capi.ERR_DTYPE, lambda: ops.PagedKVCache(codes, codes, cache.page_table)),
+        (_capi.ERR_SHAPE, lambda: ops.PagedKVCache(codes, codes, cache.page_table, scales[:1], scales)),
+        (_capi.ERR_INVALID_ARG, lambda: ops.PagedKVCache(cache.k_pages, cache.v_pages, cache.page_table, scales, scales)),
+        (_capi.ERR_DTYPE, lambda: ops.PagedKVCache(cache.k_pages, cache.v_pages, cache.page_table.long())),
+        (_capi.ERR_DTYPE, lambda: ops.PagedKVCache(cache.k_pages.float(), cache.v_pages.float(), cache.page_table)),
+        (_capi.ERR_SHAPE, lambda: ops.token_logprobs(q[0].t(), None, 1)),
+        (_capi.ERR_SHAPE, lambda: ops.token_logprobs(q[0], None, 33)),
+        (_capi.ERR_SHAPE, lambda: ops.token_logprobs(q[0], at)),
+        (_capi.ERR_DTYPE, lambda: ops.token_logprobs(codes[0, 0])),
+        (_capi.ERR_SHAPE, lambda: ops.token_logprobs(q[0], None, 3, out=ops.token_logprobs_buffers(q[0], 2))),
+    ]
+    for i, (status, call) in enumerate(calls):
+        with pytest.raises(_capi.KllmError) as e:
+            call()
+        assert e.value.status == status, (i, e.value)
+    torch.cuda.synchronize()
+
+
 # ---- a step as it is used ---------------------------------------------------------
 
 
