@@ -74,6 +74,7 @@ struct PagedAttnArgs {
   int n_heads, groups;
   int cluster;     // CTAs per cluster
   int splits;      // clusters per (token, kv head)
+  int parts_shift;  // log2(cluster * splits)
   float* part_o;   // [T, Hq, splits, D], sums of p v against the part's own max
   float* part_ml;  // [T, Hq, splits, 2] (max, sum); sum -1: the part met a bad page
   int32_t* err_flags;
@@ -179,13 +180,23 @@ __device__ __forceinline__ float exp2_approx(float x) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
 }
-// A float in the shared memory of CTA `rank` of the cluster, at this CTA's `local`.
-__device__ __forceinline__ float ld_peer(const float* local, uint32_t rank) {
+// Four floats in the shared memory of CTA `rank` of the cluster, at this CTA's
+// `local` (16-byte aligned).
+__device__ __forceinline__ float4 ld_peer(const float* local, uint32_t rank) {
   uint32_t at;
-  float v;
+  float4 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(local)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(at)
+               : "memory");
   return v;
+}
+__device__ __forceinline__ void fma4(float4& acc, float w, float4 x) {
+  acc.x = fmaf(w, x.x, acc.x);
+  acc.y = fmaf(w, x.y, acc.y);
+  acc.z = fmaf(w, x.z, acc.z);
+  acc.w = fmaf(w, x.w, acc.w);
 }
 
 // Byte offset of 16-byte chunk `ch` of row `r` in a tile of ROW-byte rows; the
@@ -209,7 +220,7 @@ template <int D, int NH>
 struct Join {
   static constexpr int kHeads = 8 * NH;
   static constexpr int kRedRow = D + 4;  // padded: eight heads' rows spread over the banks
-  static constexpr int kBytes = (kWarps * kHeads * (kRedRow + 2) + kHeads * (D + 2) + 4) * 4;
+  static constexpr int kBytes = (kWarps * kHeads * (kRedRow + 2) + kHeads * (D + 4)) * 4;
 };
 
 // One row's (or part's) share of the joined output: exp2 of its max against the
@@ -232,9 +243,9 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
   constexpr int kM = D / 16;           // m16 tiles of O^T over head_dim, k16 steps of K Q^T
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
-  const int parts = a.splits * a.cluster;
-  const int64_t t = blockIdx.x / parts;
-  const int part = static_cast<int>(blockIdx.x - t * parts);
+  const int parts = 1 << a.parts_shift;  // clusters and splits are powers of two
+  const int64_t t = blockIdx.x >> a.parts_shift;
+  const int part = blockIdx.x & (parts - 1);
   const int g = blockIdx.y;
   const int G = a.groups;
   if (threadIdx.x == 0) s_bad = 0;
@@ -605,7 +616,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
   float* red_o = reinterpret_cast<float*>(smem);
   float* red_ml = red_o + kWarps * J::kHeads * J::kRedRow;
   float* cta_o = red_ml + kWarps * J::kHeads * 2;  // [heads][D]
-  float* cta_ml = cta_o + J::kHeads * D;           // [heads][2], then the bad mark
+  float* cta_ml = cta_o + J::kHeads * D;           // [heads][4]: max, sum, the bad mark
   const float back = I8 ? vref : 1.f;
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
@@ -629,71 +640,72 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
   __syncthreads();
   bool any_bad = s_bad != 0;
   if (any_bad && threadIdx.x == 0 && g == 0) set_flag(a.err_flags, KLLM_B200_FLAG_BAD_PAGE);
-  // Head `head` of this cluster's positions: the output itself, or its share of it.
+  // Four dims of head `head` over this cluster's positions: of the output itself, or its share of it.
   const bool whole = per_part * a.cluster >= all_tiles;
-  auto finish = [&](int head, int d, float acc, float top, float sum) {
+  auto finish = [&](int head, int d, float4 acc, float top, float sum) {
     if (whole) {
-      out_t[head * D + d] = __float2half_rn(any_bad ? 0.f : acc / sum);
+      uint2 v;
+      v.x = f2_to_h2(any_bad ? 0.f : acc.x / sum, any_bad ? 0.f : acc.y / sum);
+      v.y = f2_to_h2(any_bad ? 0.f : acc.z / sum, any_bad ? 0.f : acc.w / sum);
+      *reinterpret_cast<uint2*>(out_t + head * D + d) = v;
     } else {
       const int64_t prow = (t * a.n_heads + static_cast<int64_t>(g) * G + head) * a.splits + cluster_part;
-      a.part_o[prow * D + d] = acc;
+      *reinterpret_cast<float4*>(a.part_o + prow * D + d) = acc;
       if (d == 0) {
         a.part_ml[prow * 2] = top;
         a.part_ml[prow * 2 + 1] = any_bad ? -1.f : sum;
       }
     }
   };
-  for (int idx = threadIdx.x; idx < G * D; idx += kThreads) {
-    const int head = idx / D, d = idx - head * D;
+  for (int quad = threadIdx.x; quad < G * D / 4; quad += kThreads) {
+    const int head = quad / (D / 4), d = quad % (D / 4) * 4;
+    float2 ml[kWarps];
+    float4 x[kWarps];
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) M = fmaxf(M, red_ml[(w * J::kHeads + head) * 2]);
-    float L = 0.f, acc = 0.f;
+    for (int w = 0; w < kWarps; ++w) {
+      ml[w] = *reinterpret_cast<const float2*>(red_ml + (w * J::kHeads + head) * 2);
+      x[w] = *reinterpret_cast<const float4*>(red_o + (w * J::kHeads + head) * J::kRedRow + d);
+      M = fmaxf(M, ml[w].x);
+    }
+    float L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      // a warp without tiles holds zeros and weight 0
-      const float x = join_weight(red_ml[(w * J::kHeads + head) * 2], M);
-      L += red_ml[(w * J::kHeads + head) * 2 + 1] * x;
-      acc += red_o[(w * J::kHeads + head) * J::kRedRow + d] * x;
+      const float f = join_weight(ml[w].x, M);  // a warp without tiles holds zeros and weight 0
+      L = fmaf(f, ml[w].y, L);
+      fma4(acc, f, x[w]);
     }
     if (a.cluster == 1) {
       finish(head, d, acc, M, L);
     } else {
-      cta_o[idx] = acc;
-      if (d == 0) {
-        cta_ml[2 * head] = M;
-        cta_ml[2 * head + 1] = L;
-      }
+      *reinterpret_cast<float4*>(cta_o + head * D + d) = acc;
+      if (d == 0) *reinterpret_cast<float4*>(cta_ml + 4 * head) = make_float4(M, L, any_bad ? 1.f : 0.f, 0.f);
     }
   }
   if (a.cluster == 1) return;
-  if (threadIdx.x == 0) cta_ml[2 * J::kHeads] = any_bad ? 1.f : 0.f;
   cluster_sync();
-  const int rank = part - cluster_part * a.cluster;
-  for (int c = 0; c < a.cluster; ++c) any_bad |= ld_peer(cta_ml + 2 * J::kHeads, c) != 0.f;
-  for (int idx = rank * kThreads + threadIdx.x; idx < G * D; idx += a.cluster * kThreads) {
-    const int head = idx / D, d = idx - head * D;
-    float pm[kMaxCluster], pl[kMaxCluster], po[kMaxCluster];
+  const int rank = part & (a.cluster - 1);
+  for (int quad = threadIdx.x * a.cluster + rank; quad < G * D / 4; quad += a.cluster * kThreads) {
+    const int head = quad / (D / 4), d = quad % (D / 4) * 4;
+    float4 ml[kMaxCluster], x[kMaxCluster];
 #pragma unroll
     for (int c = 0; c < kMaxCluster; ++c) {
-      if (c < a.cluster) {
-        pm[c] = ld_peer(cta_ml + 2 * head, c);
-        pl[c] = ld_peer(cta_ml + 2 * head + 1, c);
-        po[c] = ld_peer(cta_o + idx, c);
-      }
+      ml[c] = c < a.cluster ? ld_peer(cta_ml + 4 * head, c) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      x[c] = c < a.cluster ? ld_peer(cta_o + head * D + d, c) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    float M = -INFINITY, L = 0.f, acc = 0.f;
+    float M = -INFINITY, L = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int c = 0; c < kMaxCluster; ++c) {
-      if (c < a.cluster) M = fmaxf(M, pm[c]);
+      M = fmaxf(M, ml[c].x);
+      any_bad |= ml[c].z != 0.f;
     }
 #pragma unroll
     for (int c = 0; c < kMaxCluster; ++c) {
-      if (c < a.cluster) {
-        const float x = join_weight(pm[c], M);
-        L += pl[c] * x;
-        acc += po[c] * x;
-      }
+      const float f = join_weight(ml[c].x, M);
+      L = fmaf(f, ml[c].y, L);
+      fma4(acc, f, x[c]);
     }
     finish(head, d, acc, M, L);
   }
@@ -899,6 +911,7 @@ int attention_paged(const void* q, int64_t q_stride, const kllm_b200_paged_cache
   a.groups = static_cast<int>(n_heads / a.view.n_kv_heads);
   a.cluster = split.cluster;
   a.splits = static_cast<int>(splits);
+  while ((1 << a.parts_shift) < a.cluster * a.splits) ++a.parts_shift;
   a.err_flags = err_flags;
   a.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
   if (splits > 1) {
