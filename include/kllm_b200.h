@@ -361,7 +361,9 @@ int kllm_b200_qkv_norm_rope_kv_append_paged(
  * The same for v. A position at or past out_max_seq sets
  * KLLM_B200_FLAG_BAD_POSITION, a slot outside [0, n_out_slots)
  * KLLM_B200_FLAG_BAD_SLOT. Rows of padding or flagged tokens, and all others
- * of the outputs, stay as they were. Outputs 16-byte aligned. */
+ * of the outputs, stay as they were. Two tokens of one call must not name the
+ * same output row (unless they read the same one). Outputs 16-byte aligned,
+ * not overlapping the pages or one another. */
 int kllm_b200_kv_read_paged(const kllm_b200_paged_cache* cache, const int32_t* positions, const int32_t* seqs,
                             int64_t n_tokens, const int32_t* out_slots, int64_t n_out_slots, int64_t out_max_seq,
                             void* k_out, void* v_out, int32_t* err_flags, void* stream);

@@ -138,7 +138,8 @@ __device__ __forceinline__ void lds8(const float* p, float (&f)[8]) {
 // token's. Many tokens want warps more than registers: 16384 tokens of 96
 // heads of 128, int8, 148 us held to 9 CTAs per SM, 164 at the 7 that fit
 // unheld (103 us of HBM time; the rest is issue, about 290 instructions for
-// four heads, and the wait for the first loads of a warp).
+// four heads, and the wait for a warp's first loads: CTAs that stay and load
+// their next token beside the present one took 188 us).
 template <int D, bool I8, int U, bool SHARED>
 __global__ void __launch_bounds__(kThreads, SHARED && U > 1 ? (I8 ? 9 : 8) : 1) qkv_norm_rope_append_paged_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int L = D / 16;    // lanes of one head
@@ -379,81 +380,63 @@ __device__ __forceinline__ void store32(__half* p, bool aligned, uint4 lo, uint4
 
 // A CTA reads one kv head of a block of consecutive tokens, so consecutive
 // positions are consecutive rows of a page and of a head-major output. A lane
-// takes 16 bytes of a cached row of K and the same of V, of U tokens.
-template <int D, bool I8, int U>
+// takes 16 bytes of a cached row of K and the same of V. 32 x 2048 positions of
+// 32 heads of 128: int8 258 us (0.96 of the copy rate), fp16 337 us (0.97); two
+// tokens a lane took 269 us, heads before tokens 306 us.
+template <int D, bool I8>
 __global__ void __launch_bounds__(kReadThreads) kv_read_paged_kernel(const __grid_constant__ ReadArgs a) {
   constexpr int L = I8 ? D / 16 : D / 8;  // lanes of one row
-  constexpr int kRows = kReadThreads / L;
   grid_dep_wait();
   grid_dep_launch();
   const int h = blockIdx.y, hkv = a.view.n_kv_heads;
   const int c = threadIdx.x % L;
-  const int64_t t0 = static_cast<int64_t>(blockIdx.x) * (kRows * U) + threadIdx.x / L;
-  int64_t src[U], dst[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const int64_t t = t0 + u * kRows;
-    src[u] = -1;
-    if (t >= a.n_tokens) continue;
-    const int pos = __ldg(a.positions + t), seq = __ldg(a.seqs + t);
-    int flag;
-    const TokenState state = token_state(a.view, pos, seq, flag);
-    if (state == kTokenPadding) continue;
-    int64_t row = t * hkv + h;
-    if (a.out_slots != nullptr) {
-      const int slot = __ldg(a.out_slots + t);
-      if (pos >= a.out_max_seq) flag |= KLLM_B200_FLAG_BAD_POSITION;
-      if (slot < 0 || slot >= a.n_out_slots) flag |= KLLM_B200_FLAG_BAD_SLOT;
-      row = (static_cast<int64_t>(slot) * hkv + h) * a.out_max_seq + pos;
-    }
-    int page = 0;
-    if (state == kTokenOk) {
-      page = __ldg(a.view.table + seq * a.view.max_pages + (pos >> a.view.page_shift));
-      if (!page_ok(a.view, page)) flag |= KLLM_B200_FLAG_BAD_PAGE;
-    }
-    if (flag != 0) {
-      if (h == 0 && c == 0) set_flag(a.err_flags, flag);
-      continue;
-    }
-    dst[u] = row;
-    src[u] = ((static_cast<int64_t>(page) * hkv + h) << a.view.page_shift) + (pos & ((1 << a.view.page_shift) - 1));
+  const int64_t t = static_cast<int64_t>(blockIdx.x) * (kReadThreads / L) + threadIdx.x / L;
+  if (t >= a.n_tokens) return;
+  const int pos = __ldg(a.positions + t), seq = __ldg(a.seqs + t);
+  int flag;
+  const TokenState state = token_state(a.view, pos, seq, flag);
+  if (state == kTokenPadding) return;
+  int64_t to = t * hkv + h;
+  if (a.out_slots != nullptr) {
+    const int slot = __ldg(a.out_slots + t);
+    if (pos >= a.out_max_seq) flag |= KLLM_B200_FLAG_BAD_POSITION;
+    if (slot < 0 || slot >= a.n_out_slots) flag |= KLLM_B200_FLAG_BAD_SLOT;
+    to = (static_cast<int64_t>(slot) * hkv + h) * a.out_max_seq + pos;
   }
-  uint4 kw[U], vw[U];
-  float ks[U], vs[U];
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (src[u] < 0) continue;
-    const int64_t at = src[u] * (I8 ? D : 2 * D) + 16 * c;
-    kw[u] = ld_stream(static_cast<const char*>(a.k_pages) + at);
-    vw[u] = ld_stream(static_cast<const char*>(a.v_pages) + at);
-    if (I8) {
-      ks[u] = __ldg(a.k_scales + src[u]);
-      vs[u] = __ldg(a.v_scales + src[u]);
-    }
+  int page = 0;
+  if (state == kTokenOk) {
+    page = __ldg(a.view.table + seq * a.view.max_pages + (pos >> a.view.page_shift));
+    if (!page_ok(a.view, page)) flag |= KLLM_B200_FLAG_BAD_PAGE;
   }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    if (src[u] < 0) continue;
-    if (I8) {
-      uint4 lo, hi;
-      dequant16(kw[u], ks[u], lo, hi);
-      store32(a.k_out + dst[u] * D + 16 * c, a.wide, lo, hi);
-      dequant16(vw[u], vs[u], lo, hi);
-      store32(a.v_out + dst[u] * D + 16 * c, a.wide, lo, hi);
-    } else {
-      st_plain(a.k_out + dst[u] * D + 8 * c, kw[u]);
-      st_plain(a.v_out + dst[u] * D + 8 * c, vw[u]);
-    }
+  if (flag != 0) {
+    if (h == 0 && c == 0) set_flag(a.err_flags, flag);
+    return;
+  }
+  const int64_t from =
+      ((static_cast<int64_t>(page) * hkv + h) << a.view.page_shift) + (pos & ((1 << a.view.page_shift) - 1));
+  const int64_t at = from * (I8 ? D : 2 * D) + 16 * c;
+  const uint4 k = ld_stream(static_cast<const char*>(a.k_pages) + at);
+  const uint4 v = ld_stream(static_cast<const char*>(a.v_pages) + at);
+  if (I8) {
+    const float ks = __ldg(a.k_scales + from), vs = __ldg(a.v_scales + from);
+    uint4 lo, hi;
+    dequant16(k, ks, lo, hi);
+    store32(a.k_out + to * D + 16 * c, a.wide, lo, hi);
+    dequant16(v, vs, lo, hi);
+    store32(a.v_out + to * D + 16 * c, a.wide, lo, hi);
+  } else {
+    st_plain(a.k_out + to * D + 8 * c, k);
+    st_plain(a.v_out + to * D + 8 * c, v);
   }
 }
 
-template <int D, bool I8, int U>
+template <int D, bool I8>
 int launch_read(const ReadArgs& a, const LaunchOpts& o) {
-  constexpr int kTokens = kReadThreads / (I8 ? D / 16 : D / 8) * U;
+  constexpr int kTokens = kReadThreads / (I8 ? D / 16 : D / 8);
   const int64_t blocks = (a.n_tokens + kTokens - 1) / kTokens;
   if (blocks > 0x7fffffffLL) return fail(KLLM_B200_ERR_SHAPE, "kv_read_paged: too many tokens");
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.view.n_kv_heads));
-  return launch_status(launch(kv_read_paged_kernel<D, I8, U>, grid, dim3(kReadThreads), 0, o.stream, o.pdl, a),
+  return launch_status(launch(kv_read_paged_kernel<D, I8>, grid, dim3(kReadThreads), 0, o.stream, o.pdl, a),
                        "kv_read_paged");
 }
 
@@ -607,9 +590,9 @@ int kv_read_paged(const kllm_b200_paged_cache* cache, const int32_t* positions, 
   a.wide = aligned32(k_out) && aligned32(v_out);
   a.err_flags = err_flags;
   if (cache->cache_dtype == KLLM_B200_I8) {
-    return cache->head_dim == 64 ? launch_read<64, true, 1>(a, o) : launch_read<128, true, 1>(a, o);
+    return cache->head_dim == 64 ? launch_read<64, true>(a, o) : launch_read<128, true>(a, o);
   }
-  return cache->head_dim == 64 ? launch_read<64, false, 1>(a, o) : launch_read<128, false, 1>(a, o);
+  return cache->head_dim == 64 ? launch_read<64, false>(a, o) : launch_read<128, false>(a, o);
 }
 
 }  // namespace kb

@@ -68,7 +68,8 @@ def attention(q, k, v):
 
     The kernel's errors: scores from exact fp16 / code products summed in fp32
     (at most d + 4 roundings, the tensor core's accumulation counted as two
-    each) move an exponent by delta; a probability is then rounded to fp16
+    each), int8 with a query off by 2^-21 of its head's largest value, move an
+    exponent by delta; a probability is then rounded to fp16
     (E16, and an absolute 2^-25 against a largest of at least 2^11, times the
     ratio of value scales for int8, for the ones below fp16's normal range);
     sums over n positions add 2 n E32 relative to sum p |v|, the quotient and
@@ -81,7 +82,8 @@ def attention(q, k, v):
     p = torch.softmax(s, -1)
     o = torch.einsum("hj,hjd->hd", p, vv)
     size = torch.einsum("hd,hjd->hj", q.abs(), kk.abs()) / math.sqrt(d)
-    delta = (2 * (d + 8) * E32 * size.amax(-1) + 8 * E32 * (s.abs().amax(-1) + 16) + 4 * E32)[:, None]
+    digits = 2.0 ** -21 * q.abs().amax(-1) * kk.abs().sum(-1).amax(-1) / math.sqrt(d)
+    delta = (2 * (d + 8) * E32 * size.amax(-1) + digits + 8 * E32 * (s.abs().amax(-1) + 16) + 4 * E32)[:, None]
     spread = torch.einsum("hj,hjd->hd", p, vv.abs())
     vmax = vv.abs().amax((1, 2))[:, None]
     bound = (E16 + 2 * delta + 4 * n * E32) * (spread + o.abs()) + n * 2.0 ** -28 * vmax + E16 * o.abs() + TINY16
