@@ -477,6 +477,7 @@ class PagedKVCache:
         elif any(s is not None for s in scales):
             raise KllmError(_capi.ERR_INVALID_ARG, "paged cache: float16 pages take no scales")
         self._tensors = (k_pages, v_pages, k_scales, v_scales, page_table)
+        self._workspace_bytes: dict[tuple[int, int], int] = {}  # of attention_paged, by (tokens, query heads)
         n_pages, n_kv_heads, page_size, head_dim = k_pages.shape
         n_seqs, max_pages = page_table.shape
         self._descriptor = _capi.PagedCache(None, None, None, None, None, n_pages, page_size, n_kv_heads, head_dim,
@@ -658,7 +659,9 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, positions: torch.Tenso
     if workspace is not None:
         nbytes = workspace.numel() * workspace.element_size()
     elif c.max_pages * c.page_size >= _capi.PAGED_SPLIT_MIN:
-        nbytes = attention_paged_workspace_bytes(T, Hq, cache)
+        nbytes = cache._workspace_bytes.get((T, Hq))
+        if nbytes is None:
+            nbytes = cache._workspace_bytes[T, Hq] = attention_paged_workspace_bytes(T, Hq, cache)
         if nbytes:
             workspace = torch.empty(nbytes, dtype=torch.uint8, device=dev)
     _call(dev, lib.kllm_b200_attention_paged, q.data_ptr(), sq, c, positions.data_ptr(), seqs.data_ptr(), T, Hq,
