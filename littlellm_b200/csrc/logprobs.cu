@@ -30,7 +30,8 @@
 // first one's shared memory: one launch, no workspace. Bound: rows * vocab
 // values from HBM; one exponential per value (the special-function unit needs
 // three quarters of the time that fp16 values need from HBM), about five
-// issue slots per value.
+// issue slots per value. 2048 x 151936 fp16: 109 us without entries (0.87 of
+// the copy rate), 116 us with 5; one row with 20: 7.5 us.
 #include <math.h>
 
 #include "ops.cuh"
@@ -632,8 +633,10 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   }
 }
 
-// log2 of the CTAs per row: rows are split while the device has CTA slots to
-// spare and a CTA keeps at least 4096 values.
+// log2 of the CTAs per row: rows are split while their CTAs stay within two per
+// SM and each keeps at least 4096 values. Measured, us, rows of 151936 fp16 with
+// 5 entries, 1 / 2 / 4 / 8 CTAs a row: 8 rows 14.0 / 10.6 / 8.6 / 7.3, 64 rows
+// 15.2 / 11.6 / 11.5 / 12.5, 256 rows 23.3 / 24.7 / 28.0 / 39.0.
 int cluster_shift_for(int64_t rows, int64_t vocab) {
   int c = 0;
   while ((1 << c) < kMaxCluster && (rows << (c + 1)) <= 2LL * sm_count() && (vocab >> (c + 1)) >= 4096) ++c;
