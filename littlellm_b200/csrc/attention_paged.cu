@@ -238,7 +238,7 @@ __device__ __forceinline__ float join_weight(float m, float top) { return m == -
 
 // Resident CTAs that the registers are held to: int8 rows of 64 codes have the
 // shared memory for five, and want their warps (2048 sequences of up to 4095
-// positions, one box: 204 us, with four 215, with six and their spills 230).
+// positions, on one GPU: 204 us, with four 215, with six and their spills 230).
 constexpr int min_ctas(int head_dim, bool i8, int n_heads_8) { return i8 && head_dim == 64 && n_heads_8 == 1 ? 5 : 1; }
 
 template <int D, bool I8, int NH>
