@@ -1,17 +1,17 @@
 // logprobs.cu — log probability and rank of a given token, entropy and the
 // largest entries of each row of logits, from one read of the row.
 //
-// With c a reference near the row's maximum, t_i = (x_i - c) log2 e,
-// s = sum 2^t and w = sum 2^t t:
-//     log2 p_i = t_i - log2 s,   entropy = (log2 s - w / s) ln 2.
-// Each thread keeps its own (c, s, w) in fp32, moving c only when a batch of
-// values exceeds it by more than kLag (sums stay far from overflow, and what
-// the entropy's two terms cancel is bounded); threads and CTAs join by the same
-// rescaling: for c' = c + dc, s' = s 2^-dc and w' = 2^-dc (w - dc s).
-//
-// fp16 logits take t as one FMA, x log2 e - c', with the reference c' kept in
-// log2 units: the rounding of c' moves all t alike and cancels. fp32 logits
-// subtract first (x log2 e would overflow at the type's end).
+// With m the maximum, t_i = (x_i - m) log2 e, s = sum 2^t and w = sum 2^t t:
+//     log p_i = (x_i - m) - ln s,   entropy = (log2 s - w / s) ln 2.
+// All in fp32. Each thread keeps s and w against its warp's maximum m, rescaling
+// them where a batch of values brings the warp a new one (three or four times a
+// row, where a maximum per thread moves in some lane of nearly every batch);
+// warps and CTAs join the same way: for m' = m + dm (dm in log2 units),
+// s' = s 2^-dm and w' = 2^-dm (w - dm s). With m the true maximum no term of the
+// results cancels another, and the largest term is 1 exactly: a row with one
+// possible token has log probability and entropy 0. (x log2 e - m log2 e as one
+// FMA, against a reference up to 8 below the maximum, was 4% faster at 2048 x
+// 151936 and left errors of 10^-7 where the answer is 0 or nearly so.)
 //
 // Largest entries: every thread also keeps the maximum of what it read, and the
 // CTA keeps values in shared memory: all of them where they fit (kKeep vectors),
@@ -21,7 +21,8 @@
 // thread than its kept batch reaches the bound are its values read again, by the
 // whole CTA. (Reading them again in every case waits for HBM once more, behind
 // the streams of the other rows, since the rows under way do not stay in L2:
-// 2048 x 151936 fp16 with 5 / 20 entries took 120 / 137 us instead of 116 / 119.)
+// 2048 x 151936 fp16 with 5 / 20 entries took 120 / 137 us when the same sums took
+// 116 / 119 this way.)
 // A list that overflows (many equal values) is replaced by an exact scan with a
 // sorted list per warp. Entries are ordered by (value, lower id first) as one
 // 64-bit number, so equal values have one order whatever the schedule.
@@ -30,8 +31,8 @@
 // first one's shared memory: one launch, no workspace. Bound: rows * vocab
 // values from HBM; one exponential per value (the special-function unit needs
 // three quarters of the time that fp16 values need from HBM), about five
-// issue slots per value. 2048 x 151936 fp16: 109 us without entries (0.87 of
-// the copy rate), 116 us with 5; one row with 20: 7.5 us.
+// issue slots per value. 2048 x 151936 fp16: 115 us without entries (0.83 of
+// the copy rate), 122 us with 5; one row with 20: 7.7 us.
 #include <math.h>
 
 #include "ops.cuh"
@@ -47,7 +48,6 @@ constexpr int kMaxCluster = 8;
 constexpr int kListed = 512;   // values at or above the bound that fit
 constexpr int kKeep = 2560;    // vectors of a CTA that are all kept (40 KB)
 constexpr int kBatch = 4;      // 16-byte vectors a thread loads at once
-constexpr float kLag = 8.f;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
 
@@ -97,47 +97,34 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // logit never meets an infinite t.
 constexpr float kFloor = -300.f;
 
-// How a type's values relate to the reference (fp16: in log2 units, fp32: the
-// value itself).
-template <typename T>
-struct Scale;
-template <>
-struct Scale<__half> {
-  static constexpr float kUnit = kLog2e;  // reference units per logit
-  static __device__ __forceinline__ float t_of(float x, float ref) { return __fmaf_rn(x, kLog2e, -ref); }
-  static __device__ __forceinline__ float between(float from, float to) { return from - to; }
-  // log p of x, given log2 of the sum
-  static __device__ __forceinline__ float log_of(float x, float ref, float logs) { return (t_of(x, ref) - logs) * kLn2; }
-};
-template <>
-struct Scale<float> {
-  static constexpr float kUnit = 1.f;
-  static __device__ __forceinline__ float t_of(float x, float ref) { return (x - ref) * kLog2e; }
-  static __device__ __forceinline__ float between(float from, float to) { return (from - to) * kLog2e; }
-  static __device__ __forceinline__ float log_of(float x, float ref, float logs) { return (x - ref) - logs * kLn2; }
-};
+// x - m in log2 units, the argument of a power.
+__device__ __forceinline__ float t_of(float x, float m) { return (x - m) * kLog2e; }
 
-// Sums of a set of values against a reference.
-template <typename T>
+// Sums of a set of values against their maximum.
 struct Sums {
-  float ref, s, w;  // {-inf, 0, 0}: nothing yet
-  __device__ __forceinline__ void rebase(float to) {  // to >= ref
-    if (ref != to) {
-      if (ref != -INFINITY) {
-        const float d = fmaxf(Scale<T>::between(ref, to), kFloor), f = exp2_approx(d);
+  float m, s, w;  // {-inf, 0, 0}: nothing yet
+  __device__ __forceinline__ void rebase(float to) {  // to >= m
+    if (m != to) {
+      if (m != -INFINITY) {
+        const float d = fmaxf(t_of(m, to), kFloor), f = exp2_approx(d);
         w = f * fmaf(d, s, w);
         s *= f;
       }
-      ref = to;
+      m = to;
     }
   }
-  // the reference in use: 0 while everything met is -inf
-  __device__ __forceinline__ float base() const { return ref == -INFINITY ? 0.f : ref; }
-  __device__ __forceinline__ void admit(float top) {  // before adding values up to `top`
-    if (top * Scale<T>::kUnit > ref + kLag || ref == -INFINITY) rebase(fmaxf(top * Scale<T>::kUnit, ref));
+  // the maximum in use: 0 while everything met is -inf
+  __device__ __forceinline__ float base() const { return m == -INFINITY ? 0.f : m; }
+  // Before adding values up to `top`, which differs from lane to lane; m does not.
+  __device__ __forceinline__ void admit(float top) {
+    if (__any_sync(0xffffffffu, top > m)) {
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
+      rebase(top);
+    }
   }
   __device__ __forceinline__ void add(float x, float at) {
-    const float t = max_nan(Scale<T>::t_of(x, at), kFloor), e = exp2_approx(t);
+    const float t = max_nan(t_of(x, at), kFloor), e = exp2_approx(t);
     s += e;
     w = fmaf(e, t, w);
   }
@@ -182,26 +169,36 @@ struct Batch<__half> {
     }
     return static_cast<int>(__low2float(n) + __high2float(n));
   }
-  // Two values per packed fp32 instruction; s2, w2 are pairs of partial sums.
+  // Two values per packed fp32 instruction; s2, w2 are pairs of partial sums. A
+  // -inf is taken as the type's lowest value, whose power is 0 too: one packed
+  // maximum instead of a clamp of each t. Only a maximum near the lowest value
+  // itself needs the clamps.
   __device__ __forceinline__ void add(float at, unsigned long long& s2, unsigned long long& w2) const {
-    const unsigned long long scale = f32x2_pack(kLog2e, kLog2e), shift = f32x2_pack(-at, -at);
+    if (at > -65000.f) add_all<false>(at, s2, w2); else add_all<true>(at, s2, w2);
+  }
+  template <bool CLAMP>
+  __device__ __forceinline__ void add_all(float at, unsigned long long& s2, unsigned long long& w2) const {
+    const unsigned long long scale = f32x2_pack(kLog2e, kLog2e), less = f32x2_pack(-at, -at);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const uint32_t r[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const float2 x = h2_to_f2(r[i]);
-        unsigned long long t2;
-        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t2) : "l"(f32x2_pack(x.x, x.y)), "l"(scale), "l"(shift));
-        add_terms(t2, s2, w2);
+        const float2 x = __half22float2(CLAMP ? as_h2(r[i]) : __hmax2_nan(as_h2(r[i]), as_h2(0xfbfffbffu)));
+        unsigned long long d2;
+        asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d2) : "l"(f32x2_pack(x.x, x.y)), "l"(less));
+        add_terms<CLAMP>(f32x2_mul(d2, scale), s2, w2);
       }
     }
   }
+  template <bool CLAMP>
   static __device__ __forceinline__ void add_terms(unsigned long long t2, unsigned long long& s2, unsigned long long& w2) {
     float lo, hi;
     f32x2_unpack(t2, lo, hi);
-    lo = max_nan(lo, kFloor);
-    hi = max_nan(hi, kFloor);
+    if (CLAMP) {
+      lo = max_nan(lo, kFloor);
+      hi = max_nan(hi, kFloor);
+    }
     const unsigned long long e2 = f32x2_pack(exp2_approx(lo), exp2_approx(hi));
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(s2) : "l"(s2), "l"(e2));
     asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(w2) : "l"(e2), "l"(f32x2_pack(lo, hi)), "l"(w2));
@@ -239,7 +236,7 @@ struct Batch<float> {
       unpack(v[b], f);
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
-        Batch<__half>::add_terms(f32x2_pack(Scale<float>::t_of(f[i], at), Scale<float>::t_of(f[i + 1], at)), s2, w2);
+        Batch<__half>::add_terms<true>(f32x2_pack(t_of(f[i], at), t_of(f[i + 1], at)), s2, w2);
       }
     }
   }
@@ -269,9 +266,9 @@ struct Shared {
   unsigned long long listed[kListed];              // unsorted candidates
   unsigned long long joined[kMaxCluster * kMaxTop];  // first CTA: every CTA's largest entries
   uint32_t maxima[kThreads];
-  float ref[kWarps], s[kWarps], w[kWarps];
+  float m[kWarps], s[kWarps], w[kWarps];
   int above[kWarps];
-  float all_ref[kMaxCluster], all_s[kMaxCluster], all_w[kMaxCluster];  // first CTA: every CTA's sums
+  float all_m[kMaxCluster], all_s[kMaxCluster], all_w[kMaxCluster];  // first CTA: every CTA's sums
   int all_above[kMaxCluster];
   uint32_t group[64];      // maxima of 64 groups of threads
   int readers[kThreads];   // threads whose kept batch reaches the bound, from the front,
@@ -313,9 +310,8 @@ __device__ __forceinline__ Part<T> part_of(const LogprobArgs& a, int64_t r, int 
 }
 
 // Joins the sums and counts of `n` (a power of two) lanes' worth of sets; every lane gets all.
-template <typename T>
-__device__ __forceinline__ void join_lanes(Sums<T>& a, int& count, int n) {
-  float top = a.ref;
+__device__ __forceinline__ void join_lanes(Sums& a, int& count, int n) {
+  float top = a.m;
   for (int x = n / 2; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
   a.rebase(top);
   for (int x = n / 2; x > 0; x >>= 1) {
@@ -390,20 +386,17 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   const float given = asked ? to_f(p.row[token]) : INFINITY;
 
   // ---- one read: sums, count above the given token, the thread's largest batch
-  Sums<T> acc = {-INFINITY, 0.f, 0.f};
+  Sums acc = {-INFINITY, 0.f, 0.f};
   int above = 0;
   int best_at = tid;  // first vector of the kept batch
   float best = -INFINITY, second = -INFINITY, single = -INFINITY;
   const float first = tid < p.head ? to_f(p.row[tid]) : -INFINITY;
   const float last = tid < p.tail ? to_f(p.row[p.tail0 + tid]) : -INFINITY;
-  auto take = [&](float x) {
-    single = fmaxf(single, x);
-    acc.admit(x);
-    acc.add(x, acc.base());
-    above += x > given;
-  };
-  if (tid < p.head) take(first);
-  if (tid < p.tail) take(last);
+  single = fmaxf(first, last);  // -inf, which adds nothing, where there is none
+  acc.admit(single);
+  acc.add(first, acc.base());
+  acc.add(last, acc.base());
+  above += (first > given) + (last > given);
   for (int at = tid; at - tid < n_vec; at += kThreads * kBatch) {
     const Batch<T> x = next;
     load(next, at + kThreads * kBatch);
@@ -439,7 +432,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   // ---- the CTA's sums
   join_lanes(acc, above, 32);
   if (lane == 0) {
-    sh.ref[warp] = acc.ref;
+    sh.m[warp] = acc.m;
     sh.s[warp] = acc.s;
     sh.w[warp] = acc.w;
     sh.above[warp] = above;
@@ -449,17 +442,17 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   if (n_cta > 1) cluster_wait();
   __syncthreads();
   if (warp == kWarps - 1) {
-    Sums<T> all = {sh.ref[lane % kWarps], sh.s[lane % kWarps], sh.w[lane % kWarps]};
+    Sums all = {sh.m[lane % kWarps], sh.s[lane % kWarps], sh.w[lane % kWarps]};
     int n = sh.above[lane % kWarps];
     join_lanes(all, n, kWarps);
     if (lane == 0) {
       if (rank == 0) {
-        sh.all_ref[0] = all.ref;
+        sh.all_m[0] = all.m;
         sh.all_s[0] = all.s;
         sh.all_w[0] = all.w;
         sh.all_above[0] = n;
       } else {
-        push32(&sh.all_ref[rank], __float_as_uint(all.ref));
+        push32(&sh.all_m[rank], __float_as_uint(all.m));
         push32(&sh.all_s[rank], __float_as_uint(all.s));
         push32(&sh.all_w[rank], __float_as_uint(all.w));
         push32(&sh.all_above[rank], static_cast<uint32_t>(n));
@@ -595,17 +588,18 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   }
   if (rank != 0) return;
   if (warp == kWarps - 1) {
-    Sums<T> all = {sh.all_ref[lane % n_cta], sh.all_s[lane % n_cta], sh.all_w[lane % n_cta]};
+    Sums all = {sh.all_m[lane % n_cta], sh.all_s[lane % n_cta], sh.all_w[lane % n_cta]};
     int count = sh.all_above[lane % n_cta];
     join_lanes(all, count, n_cta);
     const bool nothing = all.s == 0.f;  // every logit is -inf
     const float logs = nothing ? INFINITY : log2f(all.s);  // then every log probability is -inf
+    const float lns = logs * kLn2;
     if (lane == 0) {
-      sh.ref[0] = nothing ? 0.f : all.ref;
-      sh.s[0] = logs;
+      sh.m[0] = nothing ? 0.f : all.m;
+      sh.s[0] = lns;
       if (a.tokens != nullptr) {
         if (!asked && token != -1) set_flag(a.err_flags, KLLM_B200_FLAG_BAD_TOKEN);
-        a.logprobs[r] = !asked ? 0.f : nothing ? -INFINITY : Scale<T>::log_of(given, all.ref, logs);
+        a.logprobs[r] = !asked ? 0.f : nothing ? -INFINITY : (given - all.m) - lns;
         a.ranks[r] = asked ? 1 + count : 0;
       }
       if (a.entropies != nullptr) {
@@ -629,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
     const unsigned long long e = sh.joined[tid];
     const float x = value_of(static_cast<uint32_t>(e >> 32));
     a.top_ids[r * k + tid] = static_cast<int32_t>(0xffffffffu - static_cast<uint32_t>(e));
-    a.top_logprobs[r * k + tid] = sh.s[0] == INFINITY ? -INFINITY : Scale<T>::log_of(x, sh.ref[0], sh.s[0]);
+    a.top_logprobs[r * k + tid] = sh.s[0] == INFINITY ? -INFINITY : (x - sh.m[0]) - sh.s[0];
   }
 }
 

@@ -65,10 +65,10 @@ def check(ops, x, tokens, k, err=None, **kw):
     if tokens is not None:
         close(out.logprobs, want["logprob"], lp_bound(want["logprob"]), "logprobs")
         assert torch.equal(out.ranks.cpu().long(), want["rank"].long())
-    # entropy = log s - w / s: the terms of w are weighted by their distance from a
-    # reference at most 8 below the maximum, and partly cancel log s
+    # entropy = log s - w / s, two terms of one sign: each takes the sums' error, and
+    # log s is moved by it as a whole
     h = want["entropy"]
-    close(out.entropies, h, (rel + 8 * E32) * (2 * h.abs().nan_to_num() + 24), "entropies")
+    close(out.entropies, h, (rel + 8 * E32) * (2 * h.abs().nan_to_num() + 2), "entropies")
     if k:
         assert torch.equal(out.top_ids.cpu().long(), want["ids"])
         close(out.top_logprobs, want["top"], lp_bound(want["top"]), "top_logprobs")
@@ -153,6 +153,28 @@ def test_masked_and_broken_rows(cuda, ops, dtype, vocab):
     x = x.cuda()
     for token in (0, 4, 5, vocab // 2, vocab - 1):
         check(ops, x, torch.full((12,), token, dtype=torch.int32, device="cuda"), 20)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("vocab", [1, 2, 40, 5000, 151936])
+def test_one_possible_token(cuda, ops, dtype, vocab):
+    """A grammar that leaves one token: log probability and entropy are 0, not
+    nearly 0; two tokens, one 12 above the other, keep the small one's share."""
+    rng = np.random.default_rng(vocab)
+    rows = 5
+    x = torch.full((rows, vocab), -INF, dtype=dtype)
+    at = torch.from_numpy(rng.integers(0, vocab, rows))
+    x[torch.arange(rows), at] = torch.tensor([3.3, -7.7, 0.0, 11.1, -0.013], dtype=dtype)
+    out = ops.token_logprobs(x.cuda(), at.int().cuda(), 1)
+    assert bool((out.logprobs == 0).all()) and bool((out.entropies == 0).all()) and bool((out.ranks == 1).all())
+    assert bool((out.top_logprobs == 0).all()) and torch.equal(out.top_ids[:, 0].cpu(), at.int())
+    if vocab >= 2:
+        x[torch.arange(rows), (at + vocab // 2) % vocab] = (x[torch.arange(rows), at].double() - 12).to(dtype)
+        out = ops.token_logprobs(x.cuda(), at.int().cuda(), 2)
+        want = reference(x, at.int(), 2)
+        # 1 + e^-12 in fp32: one rounding of the sum, 1 / 6e-6 of its excess; log, product and e^-12 add a few E32
+        close(out.logprobs, want["logprob"], 4 * E32, "logprobs")
+        close(out.entropies, want["entropy"], 16 * E32, "entropies")
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
