@@ -41,13 +41,14 @@
 // distributed shared memory (each takes a slice of the output), clusters
 // through the caller's workspace and a second kernel.
 //
-// Measured (B200, of the 6540 GB/s copy rate; all of a read-only stream):
-// 2048 sequences of 1 to 4095 positions, 14 heads over 2 kv heads of 64: fp16
-// 314 us (1.05), int8 199 to 215 us (0.82 to 0.88: issue, and the uneven end of
-// the ragged items). 29 sequences of 77 to 4093, 32 heads of 128, int8: 94 us
-// (0.83; 928 items on 444 CTA slots end unevenly). One token over 131072
-// positions, fp16: 17.4 us (0.59: about 6 us of dependent first loads and
-// joins); over 1001: 5.5 us.
+// Measured (B200, of the 6540 GB/s copy rate; all of a read-only stream), 14
+// heads over 2 kv heads of 64, pages of 16: 2048 sequences of 1 to 4095
+// positions fp16 314 us (1.05), int8 202 us (0.87). The int8 rest is the uneven
+// end of the ragged items and the page size: with equal lengths of 2048 it takes
+// 188 us (0.93), with pages of 64 183 (0.96), 512 x 8192 positions 175 (1.00).
+// 29 sequences of 77 to 4093, 32 heads of 128, int8: 94 us (0.83; 928 items on
+// 444 CTA slots end unevenly). One token over 131072 positions, fp16: 17.4 us
+// (0.59: about 6 us of dependent first loads and joins); over 1001: 5.5 us.
 #include <math.h>
 
 #include "paged.cuh"
