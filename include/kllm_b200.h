@@ -341,8 +341,9 @@ typedef struct kllm_b200_paged_cache {
  *   Biases of bias_dtype and norm weights [head_dim] of norm_dtype (F16 or
  *   F32), 16-byte aligned. q_out must be q itself or not overlap q, k or v.
  * A token that is padding or sets a flag leaves its q_out row and the cache
- * as they were. The (sequence, position) pairs of one call must be distinct:
- * two tokens that write one row race. */
+ * as they were. The (sequence, position) pairs of one call must be distinct,
+ * and sequences that share a page must not both append to a row of it in one
+ * call: two tokens that write one row race. */
 int kllm_b200_qkv_norm_rope_kv_append_paged(
     const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v, int64_t v_stride,
     const void* bq, const void* bk, const void* bv, int bias_dtype, const void* q_norm, const void* k_norm,
@@ -374,7 +375,7 @@ int kllm_b200_kv_read_paged(const kllm_b200_paged_cache* cache, const int32_t* p
  * k_j / sqrt(head_dim)), kv head h / (n_heads / n_kv_heads). Scores, softmax
  * statistics and sums in fp32; the probabilities enter the product with v as
  * fp16. q and out fp16 with q_stride and out_stride elements between tokens
- * (multiples of 8), 16-byte aligned, not overlapping. At most 16 query heads
+ * (multiples of 8), 16-byte aligned, not overlapping (out == q is refused). At most 16 query heads
  * per kv head. Each token is attended on its own (several tokens of one
  * sequence are allowed; each reads the sequence's pages again). Rows of
  * padding or flagged tokens become zeros. A cached row beyond positions[t] is

@@ -794,7 +794,7 @@ int check_heads(const char* what, int64_t n_tokens, int64_t n_heads, int64_t hkv
   if (n_heads / hkv > kMaxGroups) {
     return fail(KLLM_B200_ERR_SHAPE, "%s: more than %d query heads per kv head", what, kMaxGroups);
   }
-  if (n_tokens * kMaxSplits * kMaxCluster > 0x7fffffffLL) return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
+  if (n_tokens > 0x7fffffffLL / (kMaxSplits * kMaxCluster)) return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
   return KLLM_B200_OK;
 }
 
@@ -902,6 +902,7 @@ int attention_paged(const void* q, int64_t q_stride, const kllm_b200_paged_cache
   if (workspace_bytes > 0 && (!workspace || !aligned16(workspace))) {
     return fail(KLLM_B200_ERR_ALIGN, "%s: workspace must be non-null and 16-byte aligned", what);
   }
+  if (q == out) return fail(KLLM_B200_ERR_INVALID_ARG, "%s: out must not overlap q", what);
   const Split split = preferred_split(n_tokens * a.view.n_kv_heads, a.view.capacity, D,
                                       cache->cache_dtype == KLLM_B200_I8, n_heads / a.view.n_kv_heads);
   int64_t splits = split.splits;

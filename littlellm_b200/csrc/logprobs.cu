@@ -667,7 +667,7 @@ int token_logprobs(const void* logits, int dtype, int64_t rows, int64_t vocab, i
   if (rows < 0 || vocab < 0 || top_k < 0) return fail(KLLM_B200_ERR_INVALID_ARG, "%s: negative size", what);
   if (!is_float_dtype(dtype)) return fail(KLLM_B200_ERR_DTYPE, "%s: dtype %d not supported (F16, F32)", what, dtype);
   if (vocab == 0 || vocab > (1LL << 30)) return fail(KLLM_B200_ERR_SHAPE, "%s: vocab must be 1 to 2^30", what);
-  if (rows * kMaxCluster > 0x7fffffffLL) return fail(KLLM_B200_ERR_SHAPE, "%s: too many rows", what);
+  if (rows > 0x7fffffffLL / kMaxCluster) return fail(KLLM_B200_ERR_SHAPE, "%s: too many rows", what);
   if (row_stride < vocab) return fail(KLLM_B200_ERR_SHAPE, "%s: row_stride is shorter than a row", what);
   if (top_k > kMaxTop || top_k > vocab) {
     return fail(KLLM_B200_ERR_SHAPE, "%s: top_k %d must be at most %d and at most vocab", what, top_k, kMaxTop);

@@ -434,7 +434,6 @@ template <int D, bool I8>
 int launch_read(const ReadArgs& a, const LaunchOpts& o) {
   constexpr int kTokens = kReadThreads / (I8 ? D / 16 : D / 8);
   const int64_t blocks = (a.n_tokens + kTokens - 1) / kTokens;
-  if (blocks > 0x7fffffffLL) return fail(KLLM_B200_ERR_SHAPE, "kv_read_paged: too many tokens");
   const dim3 grid(static_cast<unsigned>(blocks), static_cast<unsigned>(a.view.n_kv_heads));
   return launch_status(launch(kv_read_paged_kernel<D, I8>, grid, dim3(kReadThreads), 0, o.stream, o.pdl, a),
                        "kv_read_paged");
@@ -494,6 +493,7 @@ int qkv_norm_rope_kv_append_paged(const void* q, int64_t q_stride, const void* k
   const int rc = paged_view(cache, what, &a.view);
   if (rc != KLLM_B200_OK) return rc;
   if (n_tokens == 0) return KLLM_B200_OK;
+  if (n_tokens > 0x7fffffffLL) return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
   const int64_t D = cache->head_dim, hkv = cache->n_kv_heads;
   if (n_heads == 0 || n_heads > 65535) return fail(KLLM_B200_ERR_SHAPE, "%s: 1 to 65535 query heads", what);
   if ((bq || bk || bv) && !is_float_dtype(bias_dtype)) {
@@ -570,6 +570,7 @@ int kv_read_paged(const kllm_b200_paged_cache* cache, const int32_t* positions, 
   const int rc = paged_view(cache, what, &a.view);
   if (rc != KLLM_B200_OK) return rc;
   if (n_tokens == 0) return KLLM_B200_OK;
+  if (n_tokens > 0x7fffffffLL) return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
   if (!positions || !seqs || !k_out || !v_out) return fail(KLLM_B200_ERR_INVALID_ARG, "%s: null pointer", what);
   if (out_slots && (n_out_slots == 0 || out_max_seq == 0)) return fail(KLLM_B200_ERR_SHAPE, "%s: empty output cache", what);
   if (!aligned16(k_out) || !aligned16(v_out)) {

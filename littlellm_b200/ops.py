@@ -448,6 +448,14 @@ def _all_on(device, *tensors) -> None:
             raise KllmError(_capi.ERR_INVALID_ARG, "tensors are on different devices")
 
 
+def _flags(device, err_flags) -> None:
+    """Checks an optional flag word: int32 on `device`."""
+    if err_flags is not None:
+        if err_flags.dtype is not torch.int32:
+            raise KllmError(_capi.ERR_DTYPE, "err_flags must be int32")
+        _all_on(device, err_flags)
+
+
 class PagedKVCache:
     """One layer's paged KV cache (kllm_b200_paged_cache) over given tensors.
 
@@ -566,7 +574,8 @@ def qkv_norm_rope_kv_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     [head_dim]; None: no norm) and rotate-half RoPE; k and v are appended to
     the paged cache at row positions[t] of sequence seqs[t], q goes to q_out
     (None: rotated in place). q [T, Hq, D], k and v [T, Hkv, D] fp16, tokens
-    at any stride that is a multiple of 8. positions[t] == -1 is padding."""
+    at any stride that is a multiple of 8. positions[t] == -1 is padding. No
+    two tokens of one call may write the same row of a page."""
     what = "qkv_norm_rope_kv_append_paged"
     c, dev = cache.descriptor(), cache.device
     D, Hkv = c.head_dim, c.n_kv_heads
@@ -579,7 +588,8 @@ def qkv_norm_rope_kv_append_paged(q: torch.Tensor, k: torch.Tensor, v: torch.Ten
     if not (k.shape[0] == v.shape[0] == q_out.shape[0] == T):
         raise KllmError(_capi.ERR_SHAPE, f"{what}: q, k, v and q_out must hold the same number of tokens")
     _token_index(T, dev, what, positions, seqs)
-    _all_on(dev, bq, bk, bv, q_norm, k_norm, err_flags)
+    _all_on(dev, bq, bk, bv, q_norm, k_norm)
+    _flags(dev, err_flags)
     bias = norm = F16
     if bq is not None or bk is not None or bv is not None:
         bias = _parameters(((bq, Hq * D), (bk, Hkv * D), (bv, Hkv * D)), "biases", what)
@@ -620,7 +630,8 @@ def kv_read_paged(cache: PagedKVCache, positions: torch.Tensor, seqs: torch.Tens
         raise KllmError(_capi.ERR_SHAPE, f"{what}: outputs must be {shape}")
     if k_out.dtype != torch.float16 or v_out.dtype != torch.float16:
         raise KllmError(_capi.ERR_DTYPE, f"{what}: outputs must be float16")
-    _all_on(dev, k_out, v_out, err_flags)
+    _all_on(dev, k_out, v_out)
+    _flags(dev, err_flags)
     _call(dev, lib.kllm_b200_kv_read_paged, c, positions.data_ptr(), seqs.data_ptr(), T, _ptr(out_slots), n_slots,
           max_seq, k_out.data_ptr(), v_out.data_ptr(), _ptr(err_flags))
     return k_out, v_out
@@ -642,8 +653,9 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, positions: torch.Tenso
     """Attention of single new tokens over the paged cache: token t sees
     positions 0..positions[t] of sequence seqs[t]; q and out [T, Hq, D] fp16,
     tokens at any stride that is a multiple of 8. Padding rows (position -1)
-    become zeros. ``workspace=None`` allocates the preferred one here (the C
-    entry point itself never allocates); it needs no clearing."""
+    become zeros. out must not overlap q. ``workspace=None`` allocates the
+    preferred one here (the C entry point itself never allocates); a given one
+    needs no clearing and serves one call at a time, captured ones included."""
     what = "attention_paged"
     c, dev = cache.descriptor(), cache.device
     sq = _head_rows(q, None, c.head_dim, dev, what)
@@ -654,7 +666,8 @@ def attention_paged(q: torch.Tensor, cache: PagedKVCache, positions: torch.Tenso
     if out.shape[0] != T:
         raise KllmError(_capi.ERR_SHAPE, f"{what}: q and out must hold the same number of tokens")
     _token_index(T, dev, what, positions, seqs)
-    _all_on(dev, workspace, err_flags)
+    _all_on(dev, workspace)
+    _flags(dev, err_flags)
     nbytes = 0
     if workspace is not None:
         nbytes = workspace.numel() * workspace.element_size()
@@ -698,7 +711,9 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
     """Log probability and rank of tokens[r] (int32; -1: none asked) under each
     row of logits [rows, vocab] (fp16 or fp32, rows at any stride), the row's
     entropy, and its top_k (0 to 32) largest logits as ids and log
-    probabilities, equal logits in the order of their ids."""
+    probabilities, equal logits in the order of their ids. Outputs given in
+    ``out`` that nothing asks for (logprobs and ranks without tokens) stay as
+    they were."""
     what = "token_logprobs"
     dev = logits.device
     if not logits.is_cuda:
@@ -707,6 +722,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
         raise KllmError(_capi.ERR_SHAPE, f"{what}: logits must be [rows, vocab] with contiguous rows")
     rows, vocab = logits.shape
     dtype = dtype_code(logits)
+    if not 0 <= top_k <= min(32, vocab):
+        raise KllmError(_capi.ERR_SHAPE, f"{what}: top_k {top_k} must be 0 to 32 and at most vocab")
     if out is None:
         out = token_logprobs_buffers(logits, top_k, tokens is not None)
     logprobs, ranks, entropies, top_ids, top_logprobs = out
@@ -714,7 +731,8 @@ def token_logprobs(logits: torch.Tensor, tokens: torch.Tensor | None = None, top
         _token_index(rows, dev, what, tokens)
         if logprobs is None or ranks is None:
             raise KllmError(_capi.ERR_INVALID_ARG, f"{what}: tokens need logprobs and ranks among the outputs")
-    _all_on(dev, logprobs, ranks, entropies, top_ids, top_logprobs, err_flags)
+    _all_on(dev, logprobs, ranks, entropies, top_ids, top_logprobs)
+    _flags(dev, err_flags)
     for t, kind, shape in ((logprobs, torch.float32, (rows,)), (ranks, torch.int32, (rows,)),
                            (entropies, torch.float32, (rows,)), (top_ids, torch.int32, (rows, top_k)),
                            (top_logprobs, torch.float32, (rows, top_k))):

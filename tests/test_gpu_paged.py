@@ -721,6 +721,30 @@ def test_wrapper_refusals(cuda, ops):
     torch.cuda.synchronize()
 
 
+def test_wrapper_refuses_flags_and_counts(cuda, ops):
+    from littlellm_b200 import _capi
+    cache = ops.PagedKVCache.allocate(2, 16, 2, 64, 1, 2)
+    q, kv, at = (torch.zeros(3, 4, 64, dtype=torch.float16, device="cuda"),
+                 torch.zeros(3, 2, 64, dtype=torch.float16, device="cuda"), i32([0, 1, 2]))
+    seqs = i32([0, 0, 0])
+    for flags in (torch.zeros(1, dtype=torch.uint8, device="cuda"), torch.zeros(1, device="cuda")):
+        for call in (lambda: ops.attention_paged(q, cache, at, seqs, err_flags=flags),
+                     lambda: ops.kv_read_paged(cache, at, seqs, err_flags=flags),
+                     lambda: ops.qkv_norm_rope_kv_append_paged(q, kv, kv, cache, at, seqs, 1e4, err_flags=flags),
+                     lambda: ops.token_logprobs(q[0], err_flags=flags)):
+            with pytest.raises(_capi.KllmError) as e:
+                call()
+            assert e.value.status == _capi.ERR_DTYPE
+    for k in (-1, 33, 1 << 33):
+        with pytest.raises(_capi.KllmError) as e:
+            ops.token_logprobs(q[0], None, k)
+        assert e.value.status == _capi.ERR_SHAPE
+    with pytest.raises(_capi.KllmError) as e:
+        ops.attention_paged(q, cache, at, seqs, out=q)
+    assert e.value.status == _capi.ERR_INVALID_ARG
+    torch.cuda.synchronize()
+
+
 # ---- a step as it is used ---------------------------------------------------------
 
 

@@ -122,6 +122,21 @@ def test_attention_refusals(capi):
     assert size(100_000, 8, c, n) == capi.OK and n.value == 0  # a batch that fills the device needs no parts
 
 
+@pytest.mark.parametrize("n", [1 << 31, (1 << 57) + 1, (1 << 60) + 3, (1 << 63) - 1])
+def test_counts_past_every_grid(capi, n):
+    """Also those whose products with the kernels' tile counts pass 64 bits."""
+    c = cache(capi)
+    assert append(capi, c, n=n, out=4 * P) == capi.ERR_SHAPE
+    assert read(capi, c, n=n) == capi.ERR_SHAPE
+    assert attend(capi, c, n=n, out=4 * P) == capi.ERR_SHAPE
+    assert capi.lib.kllm_b200_attention_paged_workspace_bytes(n, 8, c, ctypes.c_int64()) == capi.ERR_SHAPE
+    assert capi.lib.kllm_b200_token_logprobs(P, capi.F16, n, 100, 100, P, P, P, P, 5, P, P, None, None) == capi.ERR_SHAPE
+
+
+def test_attention_in_place_is_refused(capi):
+    assert attend(capi, cache(capi)) == capi.ERR_INVALID_ARG
+
+
 def test_logprob_refusals(capi):
     def call(**kw):
         a = dict(x=P, dtype=capi.F16, rows=2, vocab=100, stride=100, tokens=P, lp=P, ranks=P, h=P, k=5, ids=P, top=P,
