@@ -380,12 +380,14 @@ int kllm_b200_kv_read_paged(const kllm_b200_paged_cache* cache, const int32_t* p
  * sequence are allowed; each reads the sequence's pages again). Rows of
  * padding or flagged tokens become zeros. A cached row beyond positions[t] is
  * never used, whatever it holds.
- * Long sequences of small batches are split over the GPU. workspace (device,
- * 16-byte aligned) holds the parts; kllm_b200_attention_paged_workspace_bytes
- * gives its size (0 when none is needed, as for every capacity max_pages *
- * page_size below KLLM_B200_PAGED_SPLIT_MIN); a smaller or NULL workspace gives
- * coarser splits, with results that differ by rounding only. It needs no
- * clearing. Calls that share one workspace must not overlap on the GPU
+ * Long sequences of small batches are split over the GPU, and batches of more
+ * sequences than run at once are taken longest first. workspace (device,
+ * 16-byte aligned) holds the parts or the order;
+ * kllm_b200_attention_paged_workspace_bytes gives its size (0 when none is
+ * needed, as for every capacity max_pages * page_size below
+ * KLLM_B200_PAGED_SPLIT_MIN); a smaller or NULL workspace gives coarser splits,
+ * with results that differ by rounding only, or the tokens in their own order,
+ * with the same results. It needs no clearing. Calls that share one workspace must not overlap on the GPU
  * (graphs captured with the same workspace included). */
 #define KLLM_B200_PAGED_SPLIT_MIN 4096
 int kllm_b200_attention_paged_workspace_bytes(int64_t n_tokens, int64_t n_heads, const kllm_b200_paged_cache* cache,

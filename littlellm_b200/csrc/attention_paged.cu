@@ -37,18 +37,18 @@
 // scale of the value, that scale is taken relative to a power of two at or
 // above the largest the warp has met. Scores, sums and accumulators are fp32.
 //
+// Batches of more items than run at once are taken longest first.
+//
 // Join: the warps of a CTA through shared memory, the CTAs of a cluster through
 // distributed shared memory (each takes a slice of the output), clusters
 // through the caller's workspace and a second kernel.
 //
 // Measured (B200, of the 6540 GB/s copy rate; all of a read-only stream), 14
 // heads over 2 kv heads of 64, pages of 16: 2048 sequences of 1 to 4095
-// positions fp16 314 us (1.05), int8 202 us (0.87). The int8 rest is the uneven
-// end of the ragged items and the page size: with equal lengths of 2048 it takes
-// 188 us (0.93), with pages of 64 183 (0.96), 512 x 8192 positions 175 (1.00).
-// 29 sequences of 77 to 4093, 32 heads of 128, int8: 94 us (0.83; 928 items on
-// 444 CTA slots end unevenly). One token over 131072 positions, fp16: 17.4 us
-// (0.59: about 6 us of dependent first loads and joins); over 1001: 5.5 us.
+// positions fp16 309 us (1.07), int8 187 us (0.94; 1000 x 4096 positions 0.96,
+// with pages of 64 and 512 x 8192 positions 1.00). 29 sequences of 77 to 4093,
+// 32 heads of 128, int8: 79 us (0.99). One token over 131072 positions, fp16:
+// 17.3 us (0.59: about 6 us of dependent first loads and joins); over 1001: 5.4.
 #include <math.h>
 
 #include "paged.cuh"
@@ -65,6 +65,9 @@ constexpr int kMaxGroups = 16;   // query heads per kv head
 constexpr int kMaxCluster = 8;   // CTAs that join over distributed shared memory
 constexpr int kMaxSplits = 16;   // clusters of one (token, kv head)
 constexpr int kCombineWarps = 4;
+constexpr int kOrderThreads = 1024, kOrderPer = 8;  // tokens that one CTA puts in order: 8192
+constexpr int kOrderWaves = 8;                      // a batch of more waves of CTAs is not put in order
+constexpr int kLong = 2048;                         // nor one without a sequence of this many positions
 constexpr float kLift = 11.f;    // log2 of the power of a score at the reference
 constexpr float kMost = 32768.f;  // a larger power moves the reference (fp16 ends at 65504)
 
@@ -87,6 +90,7 @@ struct PagedAttnArgs {
   int parts_shift;  // log2(cluster * splits)
   float* part_o;   // [T, Hq, splits, D], sums of p v against the part's own max
   float* part_ml;  // [T, Hq, splits, 2] (max, sum); sum -1: the part met a bad page
+  int4* order;     // [T] (token, position, sequence, -), longest first, or NULL
   int32_t* err_flags;
   float scale_log2;  // log2(e) / sqrt(D)
 };
@@ -254,15 +258,26 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int gid = lane >> 2, tig = lane & 3;
   const int parts = 1 << a.parts_shift;  // clusters and splits are powers of two
-  const int64_t t = blockIdx.x >> a.parts_shift;
+  const unsigned item = blockIdx.x >> a.parts_shift, hkv = a.view.n_kv_heads;
   const int part = blockIdx.x & (parts - 1);
-  const int g = blockIdx.y;
+  const unsigned place = item / hkv;  // a token's heads side by side, neighbours in its pages (90 against 94 us at 29 x 32 heads)
+  const int g = static_cast<int>(item - place * hkv);
   const int G = a.groups;
   if (threadIdx.x == 0) s_bad = 0;
 
   grid_dep_wait();
   grid_dep_launch();
-  const int pos = a.positions[t], seq = a.seqs[t];
+  int64_t t = place;
+  int pos, seq;
+  if (a.order != nullptr) {
+    const int4 e = a.order[place];
+    t = e.x;
+    pos = e.y;
+    seq = e.z;
+  } else {
+    pos = a.positions[t];
+    seq = a.seqs[t];
+  }
   const __half* q_t = a.q + t * a.q_stride + static_cast<int64_t>(g) * G * D;
   // int8: four query values a thread and step, on their way while the page
   // table is read
@@ -781,8 +796,76 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attn_paged_combine_kernel(
   for (int k = 0; k < kPer; ++k) dst[k] = __float2half_rn(bad ? 0.f : acc[k] / L);
 }
 
-int64_t workspace_for(int64_t n_tokens, int64_t n_heads, int64_t head_dim, int64_t splits) {
-  return splits <= 1 ? 0 : n_tokens * n_heads * splits * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
+// Class of a length >= 1, longest first: eighths of octaves, by the top bits of
+// its float (exponent and three bits, 1016 for 1).
+__host__ __device__ constexpr int length_class(uint32_t float_bits) { return 255 - (static_cast<int>(float_bits >> 20) - 1016); }
+
+// Tokens, longest first, for grids of more CTAs than run at once: CTAs start in
+// the order of their index, so the last ones to start are the shortest and the
+// device stays full to the end. A counting sort by one CTA; the order within a
+// class is the atomics', which no output depends on. Costs 4 us. Without /
+// with, us, lengths of 1 to 4095: 29 sequences of 32 kv heads of 128, int8 90 /
+// 79; 14 over 2 heads of 64, 600 sequences fp16 99 / 95, int8 72 / 61; 2048
+// int8 201-215 / 186-190 (7 waves), fp16 312 / 310 (9 waves, not put in order);
+// 4096 (14 waves) int8 411 / 409. Lengths of up to 1023 keep their order (2048 sequences, fp16: 86
+// without this kernel, 90 with it, 96 sorted: the short ones, bound by latency,
+// come together at the end).
+__global__ void __launch_bounds__(kOrderThreads) attn_paged_order_kernel(const __grid_constant__ PagedAttnArgs a) {
+  __shared__ int s_first[256];
+  const int lane = threadIdx.x & 31;
+  if (threadIdx.x < 256) s_first[threadIdx.x] = 0;
+  grid_dep_wait();
+  grid_dep_launch();
+  int pos[kOrderPer], seq[kOrderPer], cls[kOrderPer], at[kOrderPer];
+  const int n = static_cast<int>(a.n_tokens);
+#pragma unroll
+  for (int u = 0; u < kOrderPer; ++u) {
+    const int t = threadIdx.x + u * kOrderThreads;
+    cls[u] = -1;
+    if (t < n) {
+      pos[u] = a.positions[t];
+      seq[u] = a.seqs[t];
+      const bool real = pos[u] >= 0 && pos[u] < a.view.capacity;  // others are done at once
+      cls[u] = real ? length_class(__float_as_uint(static_cast<float>(pos[u] + 1))) : 255;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kOrderPer; ++u) {
+    if (u * kOrderThreads >= n) break;
+    const unsigned same = __match_any_sync(0xffffffffu, cls[u]);  // one atomic per class and warp
+    const int leader = __ffs(same) - 1;
+    int base = 0;
+    if (lane == leader && cls[u] >= 0) base = atomicAdd(&s_first[cls[u]], __popc(same));
+    at[u] = __shfl_sync(0xffffffffu, base, leader) + __popc(same & ((1u << lane) - 1u));
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {  // counts to first places
+    int c[8], sum = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      c[i] = sum;
+      sum += s_first[8 * lane + i];
+    }
+    int before = sum;
+#pragma unroll
+    for (int m = 1; m < 32; m *= 2) {
+      const int x = __shfl_up_sync(0xffffffffu, before, m);
+      if (lane >= m) before += x;
+    }
+    before -= sum;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s_first[8 * lane + i] = before + c[i];
+  }
+  __syncthreads();
+  constexpr int kLongClass = length_class(0x45000000u);  // of 2048.f
+  static_assert(kLong == 2048, "its float is written above");
+  const bool sort = s_first[kLongClass + 1] > 0;  // tokens of kLong positions or more
+#pragma unroll
+  for (int u = 0; u < kOrderPer; ++u) {
+    const int t = threadIdx.x + u * kOrderThreads;
+    if (t < n) a.order[sort ? s_first[cls[u]] + at[u] : t] = make_int4(t, pos[u], seq[u], 0);
+  }
 }
 
 int check_heads(const char* what, int64_t n_tokens, int64_t n_heads, int64_t hkv) {
@@ -810,13 +893,15 @@ int check_heads(const char* what, int64_t n_tokens, int64_t n_heads, int64_t hkv
 //   fp16 128 sequences  31.1 / 30.6 / 31.5 / 46.0;  512: 87.4 / 88.0 / 100  / 166
 struct Split {
   int cluster, splits;
+  bool order;
 };
 
 template <int D, bool I8, int NH>
-Split split_of(int64_t items, int64_t capacity) {
+Split split_of(int64_t n_tokens, int64_t hkv, int64_t capacity) {
+  const int64_t items = n_tokens * hkv;
   const void* kernel = reinterpret_cast<const void*>(attn_paged_kernel<D, I8, NH>);
   const size_t smem = Ring<D, I8>::kBytes;
-  Split x = {1, 1};
+  Split x = {1, 1, false};
   (void)allow_smem(kernel, smem);  // occupancy is asked for with the opt-in in place
   for (int c = kMaxCluster; c > 1; c /= 2) {
     if (capacity < c * kWarps * kTile) continue;
@@ -829,16 +914,25 @@ Split split_of(int64_t items, int64_t capacity) {
     }
     break;
   }
+  // more than one wave, few enough that its last one counts
+  const int64_t slots = static_cast<int64_t>(sm_count()) * resident_ctas_raw(kernel, kThreads, smem);
+  x.order = x.cluster == 1 && items > slots && items <= kOrderWaves * slots && n_tokens > 1 &&
+            n_tokens <= kOrderThreads * kOrderPer && capacity >= KLLM_B200_PAGED_SPLIT_MIN;
   return x;
 }
 
-Split preferred_split(int64_t items, int64_t capacity, int64_t head_dim, bool i8, int64_t groups) {
-  if (head_dim == 64) {
-    if (i8) return groups <= 8 ? split_of<64, true, 1>(items, capacity) : split_of<64, true, 2>(items, capacity);
-    return groups <= 8 ? split_of<64, false, 1>(items, capacity) : split_of<64, false, 2>(items, capacity);
-  }
-  if (i8) return groups <= 8 ? split_of<128, true, 1>(items, capacity) : split_of<128, true, 2>(items, capacity);
-  return groups <= 8 ? split_of<128, false, 1>(items, capacity) : split_of<128, false, 2>(items, capacity);
+Split preferred_split(int64_t n_tokens, int64_t n_heads, const PagedView& view, int64_t head_dim, bool i8) {
+  const auto pick = [&](auto narrow, auto wide) {
+    return (n_heads / view.n_kv_heads <= 8 ? narrow : wide)(n_tokens, view.n_kv_heads, view.capacity);
+  };
+  if (head_dim == 64) return i8 ? pick(split_of<64, true, 1>, split_of<64, true, 2>) : pick(split_of<64, false, 1>, split_of<64, false, 2>);
+  return i8 ? pick(split_of<128, true, 1>, split_of<128, true, 2>) : pick(split_of<128, false, 1>, split_of<128, false, 2>);
+}
+
+// The workspace: parts to join, or the order of the tokens; never both.
+int64_t workspace_for(int64_t n_tokens, int64_t n_heads, int64_t head_dim, const Split& split) {
+  if (split.order) return n_tokens * static_cast<int64_t>(sizeof(int4));
+  return split.splits <= 1 ? 0 : n_tokens * n_heads * split.splits * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
 template <int D, bool I8, int NH>
@@ -849,8 +943,14 @@ int launch_attention(const PagedAttnArgs& a, const LaunchOpts& o) {
   auto kernel = attn_paged_kernel<D, I8, NH>;
   cudaError_t err = allow_smem(reinterpret_cast<const void*>(kernel), smem);
   if (err != cudaSuccess) return launch_status(err, "attention_paged: shared memory opt-in");
-  const dim3 grid(static_cast<unsigned>(a.n_tokens * a.splits * a.cluster), static_cast<unsigned>(a.view.n_kv_heads));
-  err = a.cluster == 1 ? launch(kernel, grid, dim3(kThreads), smem, o.stream, o.pdl, a)
+  const int64_t ctas = a.n_tokens * a.view.n_kv_heads * a.splits * a.cluster;
+  if (ctas > 0x7fffffffLL) return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
+  const dim3 grid(static_cast<unsigned>(ctas));
+  if (a.order != nullptr) {
+    err = launch(attn_paged_order_kernel, dim3(1), dim3(kOrderThreads), 0, o.stream, o.pdl, a);
+    if (err != cudaSuccess) return launch_status(err, what);
+  }
+  err = a.cluster == 1 ? launch(kernel, grid, dim3(kThreads), smem, o.stream, o.pdl || a.order != nullptr, a)
                        : launch_clustered(kernel, grid, dim3(kThreads), smem, o.stream, o.pdl, a.cluster, a);
   const int rc = launch_status(err, what);
   if (rc != KLLM_B200_OK || a.splits == 1) return rc;
@@ -875,9 +975,8 @@ int attention_paged_workspace_bytes(int64_t n_tokens, int64_t n_heads, const kll
   int rc = paged_view(cache, what, &view);
   if (rc == KLLM_B200_OK) rc = check_heads(what, n_tokens, n_heads, view.n_kv_heads);
   if (rc != KLLM_B200_OK || n_tokens == 0) return rc;
-  const Split split = preferred_split(n_tokens * view.n_kv_heads, view.capacity, cache->head_dim,
-                                      cache->cache_dtype == KLLM_B200_I8, n_heads / view.n_kv_heads);
-  *bytes = workspace_for(n_tokens, n_heads, cache->head_dim, split.splits);
+  *bytes = workspace_for(n_tokens, n_heads, cache->head_dim,
+                         preferred_split(n_tokens, n_heads, view, cache->head_dim, cache->cache_dtype == KLLM_B200_I8));
   return KLLM_B200_OK;
 }
 
@@ -903,10 +1002,10 @@ int attention_paged(const void* q, int64_t q_stride, const kllm_b200_paged_cache
     return fail(KLLM_B200_ERR_ALIGN, "%s: workspace must be non-null and 16-byte aligned", what);
   }
   if (q == out) return fail(KLLM_B200_ERR_INVALID_ARG, "%s: out must not overlap q", what);
-  const Split split = preferred_split(n_tokens * a.view.n_kv_heads, a.view.capacity, D,
-                                      cache->cache_dtype == KLLM_B200_I8, n_heads / a.view.n_kv_heads);
-  int64_t splits = split.splits;
-  while (workspace_for(n_tokens, n_heads, D, splits) > (workspace ? workspace_bytes : 0)) splits /= 2;
+  Split split = preferred_split(n_tokens, n_heads, a.view, D, cache->cache_dtype == KLLM_B200_I8);
+  const auto fits = [&] { return workspace_for(n_tokens, n_heads, D, split) <= (workspace ? workspace_bytes : 0); };
+  if (split.order && !fits()) split.order = false;
+  while (!fits()) split.splits /= 2;
   a.q = static_cast<const __half*>(q);
   a.q_stride = q_stride;
   a.out = static_cast<__half*>(out);
@@ -921,13 +1020,14 @@ int attention_paged(const void* q, int64_t q_stride, const kllm_b200_paged_cache
   a.n_heads = static_cast<int>(n_heads);
   a.groups = static_cast<int>(n_heads / a.view.n_kv_heads);
   a.cluster = split.cluster;
-  a.splits = static_cast<int>(splits);
+  a.splits = split.splits;
   while ((1 << a.parts_shift) < a.cluster * a.splits) ++a.parts_shift;
   a.err_flags = err_flags;
   a.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));
-  if (splits > 1) {
+  if (split.order) a.order = static_cast<int4*>(workspace);
+  if (split.splits > 1) {
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + n_tokens * n_heads * splits * D;
+    a.part_ml = a.part_o + n_tokens * n_heads * split.splits * D;
   }
   if (cache->cache_dtype == KLLM_B200_I8) return D == 64 ? launch_groups<64, true>(a, o) : launch_groups<128, true>(a, o);
   return D == 64 ? launch_groups<64, false>(a, o) : launch_groups<128, false>(a, o);

@@ -721,6 +721,84 @@ def test_wrapper_refusals(cuda, ops):
     torch.cuda.synchronize()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hkv,d,n,longest", [
+    (2, 64, 400, 4096),    # GQA heads
+    (2, 64, 1025, 4095),   # one token past a thread's first
+    (1, 64, 3001, 2600),
+    (32, 128, 29, 4093),   # many heads, few tokens
+    (3, 128, 513, 2048),   # just long enough to be put in order
+    (3, 128, 513, 2047),   # and not
+    (2, 64, 1024, 1),      # one position each
+])
+def test_attention_longest_first(cuda, ops, dtype, hkv, d, n, longest):
+    """Batches of more items than run at once: the order in which they are
+    taken changes no bit, with padding and bad tokens among them."""
+    rng = np.random.default_rng(n + longest)
+    page, n_pages, hq = 16, 40, 2 * hkv
+    table = rng.integers(0, n_pages, (n, 256)).astype(np.int32)  # sequences share pages
+    cache, k, v = pu.random_cache(rng, ops, dtype, n_pages, hkv, page, d, table)
+    positions = rng.integers(0, longest, n)
+    positions[rng.integers(0, n, 2)] = longest - 1
+    seqs = rng.permutation(n)
+    q = randh(rng, n, hq, d, scale=1.5).cuda()
+    nbytes = ops.attention_paged_workspace_bytes(n, hq, cache)
+    # in order from one to eight waves of CTAs; fp16 rows of 128 leave room for
+    # one CTA of 128 KB per SM, so 1539 items are ten waves of 148
+    waves_past = dtype == torch.float16 and hkv * n > 8 * 148 and d == 128
+    assert nbytes == (0 if waves_past else 16 * n)
+    ws = torch.full((nbytes + 64,), 0x7f, dtype=torch.uint8, device="cuda")
+    sample = rng.permutation(n)[:12].tolist() + [int(positions.argmax())]
+    for bad in (False, True):
+        want_flags = 0
+        if bad:
+            positions[:5], seqs[5] = [-1, -1, 4096, -2, 2 ** 31 - 1], n
+            from littlellm_b200 import _capi
+            want_flags = _capi.FLAG_BAD_POSITION | _capi.FLAG_BAD_SEQ
+        outs = []
+        for work in (ws[:0], ws[:nbytes], None):
+            err = flags()
+            out = torch.full((n, hq, d), -5.0, dtype=torch.float16, device="cuda")
+            ops.attention_paged(q, cache, i32(positions), i32(seqs), out=out, workspace=work, err_flags=err)
+            torch.cuda.synchronize()
+            assert int(err.item()) == want_flags
+            outs.append(out)
+        assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], outs[2])
+        assert bool((ws[nbytes:] == 0x7f).all())
+        if bad:
+            assert bool((outs[0][:6] == 0).all())
+            continue
+        got = outs[0].cpu().double()
+        for t in sample:
+            p, at = int(positions[t]), int(seqs[t])
+            want, bound = pu.attention(q[t].cpu().double(), pu.rows_of(k, table, at, p + 1), pu.rows_of(v, table, at, p + 1))
+            assert ((got[t] - want).abs() <= bound).all()
+
+
+def test_attention_longest_first_in_a_graph(cuda, ops):
+    """The order is made from the positions of each replay; lengths all equal,
+    ragged, and all padding."""
+    rng = np.random.default_rng(77)
+    n, hq, hkv, d = 640, 4, 2, 64
+    table = rng.integers(0, 40, (n, 256)).astype(np.int32)
+    cache, _, _ = pu.random_cache(rng, ops, torch.int8, 40, hkv, 16, d, table)
+    q, seqs = randh(rng, n, hq, d).cuda(), i32(rng.permutation(n))
+    positions, out = i32(np.zeros(n)), torch.empty(n, hq, d, dtype=torch.float16, device="cuda")
+    ws = torch.empty(ops.attention_paged_workspace_bytes(n, hq, cache), dtype=torch.uint8, device="cuda")
+    assert ws.numel() == 16 * n
+    ops.attention_paged(q, cache, positions, seqs, out=out, workspace=ws)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.attention_paged(q, cache, positions, seqs, out=out, workspace=ws)
+    for p in (np.full(n, 4095), rng.integers(-1, 4096, n), np.full(n, -1), rng.integers(0, 4096, n)):
+        positions.copy_(i32(p))
+        out.fill_(-5.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.attention_paged(q, cache, positions, seqs, workspace=ws[:0]))
+
+
 def test_wrapper_refuses_flags_and_counts(cuda, ops):
     from littlellm_b200 import _capi
     cache = ops.PagedKVCache.allocate(2, 16, 2, 64, 1, 2)
