@@ -97,16 +97,23 @@ __device__ __forceinline__ float max_nan(float a, float b) {
 // logit never meets an infinite t.
 constexpr float kFloor = -300.f;
 
-// x - m in log2 units, the argument of a power.
-__device__ __forceinline__ float t_of(float x, float m) { return (x - m) * kLog2e; }
-
-// Sums of a set of values against their maximum.
+// Sums of a set of values against their maximum. A term is 2^t, t = x log2 e -
+// c, c the reference of the maximum m in log2 units. fp16 logits: c = m log2 e
+// rounded and t one FMA, off by its own rounding and, alike in every term, by
+// that of c; fp32 logits, whose product could leave the range: t = (x - m)
+// log2 e, and c stands for m itself.
+template <typename T>
 struct Sums {
+  static constexpr bool kFma = sizeof(T) == 2;
   float m, s, w;  // {-inf, 0, 0}: nothing yet
+  static __device__ __forceinline__ float term(float x, float at) {
+    return kFma ? fmaf(x, kLog2e, -__fmul_rn(at, kLog2e)) : (x - at) * kLog2e;
+  }
   __device__ __forceinline__ void rebase(float to) {  // to >= m
     if (m != to) {
       if (m != -INFINITY) {
-        const float d = fmaxf(t_of(m, to), kFloor), f = exp2_approx(d);
+        const float step = kFma ? __fsub_rn(__fmul_rn(m, kLog2e), __fmul_rn(to, kLog2e)) : (m - to) * kLog2e;
+        const float d = fmaxf(step, kFloor), f = exp2_approx(d);
         w = f * fmaf(d, s, w);
         s *= f;
       }
@@ -123,10 +130,19 @@ struct Sums {
       rebase(top);
     }
   }
-  __device__ __forceinline__ void add(float x, float at) {
-    const float t = max_nan(t_of(x, at), kFloor), e = exp2_approx(t);
+  __device__ __forceinline__ void add(float x) {
+    const float t = max_nan(term(x, base()), kFloor), e = exp2_approx(t);
     s += e;
     w = fmaf(e, t, w);
+  }
+  // Takes the reference's rounding out: every term of a value m is 2^t0 as
+  // computed, and is 1 afterwards.
+  __device__ __forceinline__ void settle() {
+    if (kFma && m != -INFINITY) {
+      const float t0 = term(m, m), unit = exp2_approx(t0);
+      w = __fsub_rn(w, __fmul_rn(t0, s)) / unit;
+      s = s / unit;
+    }
   }
 };
 
@@ -178,16 +194,17 @@ struct Batch<__half> {
   }
   template <bool CLAMP>
   __device__ __forceinline__ void add_all(float at, unsigned long long& s2, unsigned long long& w2) const {
-    const unsigned long long scale = f32x2_pack(kLog2e, kLog2e), less = f32x2_pack(-at, -at);
+    const float c = -__fmul_rn(at, kLog2e);
+    const unsigned long long scale = f32x2_pack(kLog2e, kLog2e), less = f32x2_pack(c, c);
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
       const uint32_t r[4] = {v[b].x, v[b].y, v[b].z, v[b].w};
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 x = __half22float2(CLAMP ? as_h2(r[i]) : __hmax2_nan(as_h2(r[i]), as_h2(0xfbfffbffu)));
-        unsigned long long d2;
-        asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d2) : "l"(f32x2_pack(x.x, x.y)), "l"(less));
-        add_terms<CLAMP>(f32x2_mul(d2, scale), s2, w2);
+        unsigned long long t2;
+        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t2) : "l"(f32x2_pack(x.x, x.y)), "l"(scale), "l"(less));
+        add_terms<CLAMP>(t2, s2, w2);
       }
     }
   }
@@ -236,7 +253,7 @@ struct Batch<float> {
       unpack(v[b], f);
 #pragma unroll
       for (int i = 0; i < 4; i += 2) {
-        Batch<__half>::add_terms<true>(f32x2_pack(t_of(f[i], at), t_of(f[i + 1], at)), s2, w2);
+        Batch<__half>::add_terms<true>(f32x2_pack(Sums<float>::term(f[i], at), Sums<float>::term(f[i + 1], at)), s2, w2);
       }
     }
   }
@@ -310,7 +327,8 @@ __device__ __forceinline__ Part<T> part_of(const LogprobArgs& a, int64_t r, int 
 }
 
 // Joins the sums and counts of `n` (a power of two) lanes' worth of sets; every lane gets all.
-__device__ __forceinline__ void join_lanes(Sums& a, int& count, int n) {
+template <typename T>
+__device__ __forceinline__ void join_lanes(Sums<T>& a, int& count, int n) {
   float top = a.m;
   for (int x = n / 2; x > 0; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
   a.rebase(top);
@@ -373,20 +391,28 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   const int token = a.tokens != nullptr ? a.tokens[r] : -1;
   const Part<T> p = part_of<T>(a, r, rank, cta_shift);
   const int n_vec = p.n_vec;
-  auto load = [&](Batch<T>& x, int at) {
+  // Batch i of the thread, from vector `at`; whole ones load without predicates
+  constexpr int kSpan = kThreads * kBatch;
+  const int whole = n_vec / kSpan, n_batches = (n_vec + kSpan - 1) / kSpan;
+  auto load = [&](Batch<T>& x, int i, int at) {
+    if (i < whole) {
 #pragma unroll
-    for (int b = 0; b < kBatch; ++b) {
-      const int v = at + b * kThreads;
-      x.v[b] = v < n_vec ? ld_stream(p.body + v) : Batch<T>::none();
+      for (int b = 0; b < kBatch; ++b) x.v[b] = ld_stream(p.body + at + b * kThreads);
+    } else {
+#pragma unroll
+      for (int b = 0; b < kBatch; ++b) {
+        const int v = at + b * kThreads;
+        x.v[b] = v < n_vec ? ld_stream(p.body + v) : Batch<T>::none();
+      }
     }
   };
-  Batch<T> next;
-  load(next, tid);
+  Batch<T> even, odd;
+  load(even, 0, tid);
   const bool asked = token >= 0 && token < a.vocab;
   const float given = asked ? to_f(p.row[token]) : INFINITY;
 
   // ---- one read: sums, count above the given token, the thread's largest batch
-  Sums acc = {-INFINITY, 0.f, 0.f};
+  Sums<T> acc = {-INFINITY, 0.f, 0.f};
   int above = 0;
   int best_at = tid;  // first vector of the kept batch
   float best = -INFINITY, second = -INFINITY, single = -INFINITY;
@@ -394,12 +420,10 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   const float last = tid < p.tail ? to_f(p.row[p.tail0 + tid]) : -INFINITY;
   single = fmaxf(first, last);  // -inf, which adds nothing, where there is none
   acc.admit(single);
-  acc.add(first, acc.base());
-  acc.add(last, acc.base());
+  acc.add(first);
+  acc.add(last);
   above += (first > given) + (last > given);
-  for (int at = tid; at - tid < n_vec; at += kThreads * kBatch) {
-    const Batch<T> x = next;
-    load(next, at + kThreads * kBatch);
+  auto take = [&](const Batch<T>& x, int at) {
     const float top = x.top();
     second = fmaxf(second, fminf(best, top));
     acc.admit(top);
@@ -427,6 +451,13 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
     acc.s = lo + hi;
     f32x2_unpack(w2, lo, hi);
     acc.w = lo + hi;
+  };
+  for (int i = 0, at = tid; i < n_batches; i += 2, at += 2 * kSpan) {
+    load(odd, i + 1, at + kSpan);
+    take(even, at);
+    if (i + 1 == n_batches) break;
+    load(even, i + 2, at + 2 * kSpan);
+    take(odd, at + kSpan);
   }
 
   // ---- the CTA's sums
@@ -442,7 +473,7 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   if (n_cta > 1) cluster_wait();
   __syncthreads();
   if (warp == kWarps - 1) {
-    Sums all = {sh.m[lane % kWarps], sh.s[lane % kWarps], sh.w[lane % kWarps]};
+    Sums<T> all = {sh.m[lane % kWarps], sh.s[lane % kWarps], sh.w[lane % kWarps]};
     int n = sh.above[lane % kWarps];
     join_lanes(all, n, kWarps);
     if (lane == 0) {
@@ -588,9 +619,10 @@ __global__ void __launch_bounds__(kThreads, 4) token_logprobs_kernel(const __gri
   }
   if (rank != 0) return;
   if (warp == kWarps - 1) {
-    Sums all = {sh.all_m[lane % n_cta], sh.all_s[lane % n_cta], sh.all_w[lane % n_cta]};
+    Sums<T> all = {sh.all_m[lane % n_cta], sh.all_s[lane % n_cta], sh.all_w[lane % n_cta]};
     int count = sh.all_above[lane % n_cta];
     join_lanes(all, count, n_cta);
+    all.settle();
     const bool nothing = all.s == 0.f;  // every logit is -inf
     const float logs = nothing ? INFINITY : log2f(all.s);  // then every log probability is -inf
     const float lns = logs * kLn2;
