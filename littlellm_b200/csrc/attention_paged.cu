@@ -45,8 +45,7 @@
 //
 // Measured (B200, of the 6540 GB/s copy rate; all of a read-only stream), 14
 // heads over 2 kv heads of 64, pages of 16: 2048 sequences of 1 to 4095
-// positions fp16 309 us (1.07), int8 187 us (0.94; 1000 x 4096 positions 0.96,
-// with pages of 64 and 512 x 8192 positions 1.00). 29 sequences of 77 to 4093,
+// positions fp16 309 us (1.07), int8 184 us (0.95; 1000 x 4096 positions 0.98). 29 sequences of 77 to 4093,
 // 32 heads of 128, int8: 79 us (0.99). One token over 131072 positions, fp16:
 // 17.3 us (0.59: about 6 us of dependent first loads and joins); over 1001: 5.4.
 #include <math.h>
@@ -803,13 +802,14 @@ __host__ __device__ constexpr int length_class(uint32_t float_bits) { return 255
 // Tokens, longest first, for grids of more CTAs than run at once: CTAs start in
 // the order of their index, so the last ones to start are the shortest and the
 // device stays full to the end. A counting sort by one CTA; the order within a
-// class is the atomics', which no output depends on. Costs 4 us. Without /
-// with, us, lengths of 1 to 4095: 29 sequences of 32 kv heads of 128, int8 90 /
-// 79; 14 over 2 heads of 64, 600 sequences fp16 99 / 95, int8 72 / 61; 2048
-// int8 201-215 / 186-190 (7 waves), fp16 312 / 310 (9 waves, not put in order);
-// 4096 (14 waves) int8 411 / 409. Lengths of up to 1023 keep their order (2048 sequences, fp16: 86
-// without this kernel, 90 with it, 96 sorted: the short ones, bound by latency,
-// come together at the end).
+// class is the atomics', which no output depends on. Costs 2 to 3 us (one more
+// with a match of the warp's classes before each atomic). Without / with, us,
+// lengths of 1 to 4095: 29 sequences of 32 kv heads of 128, int8 90 / 79; 14
+// over 2 heads of 64, 600 sequences fp16 99 / 95, int8 72 / 61; 2048 int8
+// 201-215 / 182-186 (6 waves), fp16 312 / 310 (9 waves, not put in order); 4096
+// (11 waves) int8 411 / 409. Lengths below kLong keep their order: 2048
+// sequences of up to 1023, fp16, 86 without this kernel, 90 with it, 96 sorted,
+// when the short ones, which latency bounds, come together at the end.
 __global__ void __launch_bounds__(kOrderThreads) attn_paged_order_kernel(const __grid_constant__ PagedAttnArgs a) {
   __shared__ int s_first[256];
   const int lane = threadIdx.x & 31;
@@ -833,11 +833,13 @@ __global__ void __launch_bounds__(kOrderThreads) attn_paged_order_kernel(const _
 #pragma unroll
   for (int u = 0; u < kOrderPer; ++u) {
     if (u * kOrderThreads >= n) break;
-    const unsigned same = __match_any_sync(0xffffffffu, cls[u]);  // one atomic per class and warp
-    const int leader = __ffs(same) - 1;
-    int base = 0;
-    if (lane == leader && cls[u] >= 0) base = atomicAdd(&s_first[cls[u]], __popc(same));
-    at[u] = __shfl_sync(0xffffffffu, base, leader) + __popc(same & ((1u << lane) - 1u));
+    const int front = __shfl_sync(0xffffffffu, cls[u], 0);  // by all lanes, before any condition on their class
+    if (__all_sync(0xffffffffu, front >= 0 && cls[u] == front)) {
+      const int base = lane == 0 ? atomicAdd(&s_first[cls[u]], 32) : 0;  // equal lengths: one atomic, not 32 in turn
+      at[u] = __shfl_sync(0xffffffffu, base, 0) + lane;
+    } else if (cls[u] >= 0) {
+      at[u] = atomicAdd(&s_first[cls[u]], 1);
+    }
   }
   __syncthreads();
   if (threadIdx.x < 32) {  // counts to first places

@@ -8,10 +8,9 @@
 // row, where a maximum per thread moves in some lane of nearly every batch);
 // warps and CTAs join the same way: for m' = m + dm (dm in log2 units),
 // s' = s 2^-dm and w' = 2^-dm (w - dm s). With m the true maximum no term of the
-// results cancels another, and the largest term is 1 exactly: a row with one
-// possible token has log probability and entropy 0. (x log2 e - m log2 e as one
-// FMA, against a reference up to 8 below the maximum, was 4% faster at 2048 x
-// 151936 and left errors of 10^-7 where the answer is 0 or nearly so.)
+// results cancels another, and the largest term is 1 (for fp16, whose exponent
+// is one FMA, once the rounding common to all terms is taken out at the end of
+// the row): a row with one possible token has log probability and entropy 0.
 //
 // Largest entries: every thread also keeps the maximum of what it read, and the
 // CTA keeps values in shared memory: all of them where they fit (kKeep vectors),
@@ -30,9 +29,13 @@
 // A row is read by a cluster of 1 to 8 CTAs whose parts are pushed to the
 // first one's shared memory: one launch, no workspace. Bound: rows * vocab
 // values from HBM; one exponential per value (the special-function unit needs
-// three quarters of the time that fp16 values need from HBM), about five
-// issue slots per value. 2048 x 151936 fp16: 115 us without entries (0.83 of
-// the copy rate), 122 us with 5; one row with 20: 7.7 us.
+// three quarters of the time that fp16 values need from HBM), about seven
+// issue slots per value. 2048 x 151936 fp16: 106 us without entries (0.90 of
+// the copy rate), 116 us with 5 (4300 warp instructions a row: keeping batches,
+// the bound, the list); one row with 20: 7.9 us. Whole batches are loaded without
+// predicates into two sets in turn (a copy of 16 registers and as many defaults
+// per batch less: 4%). CTAs that stay and load their next row's first batch while
+// they finish one took 131 us (spills).
 #include <math.h>
 
 #include "ops.cuh"
