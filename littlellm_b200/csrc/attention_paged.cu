@@ -45,9 +45,10 @@
 //
 // Measured (B200, of the 6540 GB/s copy rate; all of a read-only stream), 14
 // heads over 2 kv heads of 64, pages of 16: 2048 sequences of 1 to 4095
-// positions fp16 309 us (1.07), int8 184 us (0.95; 1000 x 4096 positions 0.98). 29 sequences of 77 to 4093,
-// 32 heads of 128, int8: 79 us (0.99). One token over 131072 positions, fp16:
-// 17.3 us (0.59: about 6 us of dependent first loads and joins); over 1001: 5.4.
+// positions fp16 309 us (1.07), int8 184 us (0.95; 1000 x 4096 positions 0.98).
+// 29 sequences of 77 to 4093, 32 heads of 128, int8: 79 us (0.99). One token
+// over 131072 positions, fp16: 17.3 us (0.59: about 6 us of dependent first
+// loads and joins); over 1001: 5.4.
 #include <math.h>
 
 #include "paged.cuh"
@@ -879,7 +880,10 @@ int check_heads(const char* what, int64_t n_tokens, int64_t n_heads, int64_t hkv
   if (n_heads / hkv > kMaxGroups) {
     return fail(KLLM_B200_ERR_SHAPE, "%s: more than %d query heads per kv head", what, kMaxGroups);
   }
-  if (n_tokens > 0x7fffffffLL / (kMaxSplits * kMaxCluster)) return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
+  // a CTA per (token, kv head) at least, all parts of few
+  if (n_tokens > 0x7fffffffLL / (kMaxSplits * kMaxCluster) || n_tokens * hkv > 0x7fffffffLL) {
+    return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
+  }
   return KLLM_B200_OK;
 }
 
@@ -945,9 +949,7 @@ int launch_attention(const PagedAttnArgs& a, const LaunchOpts& o) {
   auto kernel = attn_paged_kernel<D, I8, NH>;
   cudaError_t err = allow_smem(reinterpret_cast<const void*>(kernel), smem);
   if (err != cudaSuccess) return launch_status(err, "attention_paged: shared memory opt-in");
-  const int64_t ctas = a.n_tokens * a.view.n_kv_heads * a.splits * a.cluster;
-  if (ctas > 0x7fffffffLL) return fail(KLLM_B200_ERR_SHAPE, "%s: too many tokens", what);
-  const dim3 grid(static_cast<unsigned>(ctas));
+  const dim3 grid(static_cast<unsigned>(a.n_tokens * a.view.n_kv_heads * a.splits * a.cluster));
   if (a.order != nullptr) {
     err = launch(attn_paged_order_kernel, dim3(1), dim3(kOrderThreads), 0, o.stream, o.pdl, a);
     if (err != cudaSuccess) return launch_status(err, what);

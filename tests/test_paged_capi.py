@@ -133,6 +133,13 @@ def test_counts_past_every_grid(capi, n):
     assert capi.lib.kllm_b200_token_logprobs(P, capi.F16, n, 100, 100, P, P, P, P, 5, P, P, None, None) == capi.ERR_SHAPE
 
 
+def test_more_items_than_a_grid_holds(capi):
+    c = cache(capi, n_kv_heads=65535)
+    wide = 65535 * 64
+    assert attend(capi, c, n=1 << 20, heads=65535, qs=wide, os=wide, out=4 * P) == capi.ERR_SHAPE
+    assert capi.lib.kllm_b200_attention_paged_workspace_bytes(1 << 20, 65535, c, ctypes.c_int64()) == capi.ERR_SHAPE
+
+
 def test_attention_in_place_is_refused(capi):
     assert attend(capi, cache(capi)) == capi.ERR_INVALID_ARG
 
