@@ -57,8 +57,7 @@
 namespace kb {
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
+constexpr int kWarps = 4;        // of a CTA; 1 in the narrow form
 constexpr int kTile = 32;        // positions per warp tile
 constexpr int kStages = 2;       // tiles of the cp.async ring (3: fewer resident CTAs, 2 to 3% slower)
 constexpr int kMaxGroups = 16;   // query heads per kv head
@@ -66,8 +65,9 @@ constexpr int kMaxCluster = 8;   // CTAs that join over distributed shared memor
 constexpr int kMaxSplits = 16;   // clusters of one (token, kv head)
 constexpr int kCombineWarps = 4;
 constexpr int kOrderThreads = 1024, kOrderPer = 8;  // tokens that one CTA puts in order: 8192
-constexpr int kOrderWaves = 8;                      // a batch of more waves of CTAs is not put in order
-constexpr int kLong = 2048;                         // nor one without a sequence of this many positions
+constexpr int kOrderWaves = 8;    // a batch of more waves of CTAs is not put in order,
+constexpr int kLong = 2048;       // nor one without a sequence of this many positions
+constexpr int64_t kNarrow = 128;  // positions of capacity per wave of CTAs up to which a CTA is one warp
 constexpr float kLift = 11.f;    // log2 of the power of a score at the reference
 constexpr float kMost = 32768.f;  // a larger power moves the reference (fp16 ends at 65504)
 
@@ -221,20 +221,20 @@ __device__ __forceinline__ uint32_t swz(int r, int ch) {
   return static_cast<uint32_t>(r * ROW + ((ROW == 64 ? ch ^ ((r >> 1) & 3) : ch ^ (r & 7)) << 4));
 }
 
-template <int D, bool I8>
+template <int D, bool I8, int W>
 struct Ring {
   static constexpr int kRow = I8 ? D : 2 * D;  // bytes of a cached row
   static constexpr int kTileBytes = kTile * kRow;
   static constexpr int kStageBytes = 2 * kTileBytes + (I8 ? 2 * kTile * 4 : 0);  // K, V, their scales
-  static constexpr int kBytes = kWarps * kStages * kStageBytes;
+  static constexpr int kBytes = W * kStages * kStageBytes;
 };
 
 // Shared memory of the join, over the idle rings.
-template <int D, int NH>
+template <int D, int NH, int W>
 struct Join {
   static constexpr int kHeads = 8 * NH;
   static constexpr int kRedRow = D + 4;  // padded: eight heads' rows spread over the banks
-  static constexpr int kBytes = (kWarps * kHeads * (kRedRow + 2) + kHeads * (D + 4)) * 4;
+  static constexpr int kBytes = (W * kHeads * (kRedRow + 2) + kHeads * (D + 4)) * 4;
 };
 
 // One row's (or part's) share of the joined output: exp2 of its max against the
@@ -244,11 +244,19 @@ __device__ __forceinline__ float join_weight(float m, float top) { return m == -
 // Resident CTAs that the registers are held to: int8 rows of 64 codes have the
 // shared memory for five, and want their warps (2048 sequences of up to 4095
 // positions, on one GPU: 204 us, with four 215, with six and their spills 230).
-constexpr int min_ctas(int head_dim, bool i8, int n_heads_8) { return i8 && head_dim == 64 && n_heads_8 == 1 ? 5 : 1; }
+constexpr int min_ctas(int head_dim, bool i8, int n_heads_8, int warps) {
+  return warps == kWarps && i8 && head_dim == 64 && n_heads_8 == 1 ? 5 : 1;
+}
 
-template <int D, bool I8, int NH>
-__global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
-  using R = Ring<D, I8>;
+template <int D, bool I8, int NH, int W>
+constexpr size_t smem_bytes() {
+  return Ring<D, I8, W>::kBytes > Join<D, NH, W>::kBytes ? Ring<D, I8, W>::kBytes : Join<D, NH, W>::kBytes;
+}
+
+template <int D, bool I8, int NH, int W>
+__global__ void __launch_bounds__(W * 32, min_ctas(D, I8, NH, W)) attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
+  using R = Ring<D, I8, W>;
+  constexpr int kThreads = W * 32;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int s_bad;
   constexpr int kRow = R::kRow;
@@ -306,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
   if (cluster_part * a.cluster * per_part >= all_tiles) return;  // nothing left for this cluster
   const int tile0 = min(part * per_part, all_tiles);
   const int n_tiles = min(per_part, all_tiles - tile0);
-  const int my_tiles = n_tiles > warp ? (n_tiles - warp + kWarps - 1) / kWarps : 0;
+  const int my_tiles = n_tiles > warp ? (n_tiles - warp + W - 1) / W : 0;
 
   const int shift = a.view.page_shift, mask = (1 << shift) - 1;
   const int32_t* table = a.view.table + seq * a.view.max_pages;
@@ -315,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
 
   // The page of this lane's position of warp tile i (-1 past the end).
   auto page_of = [&](int i) {
-    const int j = (tile0 + warp + i * kWarps) * kTile + lane;
+    const int j = (tile0 + warp + i * W) * kTile + lane;
     return i < my_tiles && j < n ? __ldg(table + (j >> shift)) : -1;
   };
   const int lane_row = lane / kChunks, lane_ch = lane % kChunks;
@@ -325,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
   // zero-filled, so no stale bits reach the products.
   auto issue = [&](int i, int page, int st) {
     if (i < my_tiles) {
-      const int j0 = (tile0 + warp + i * kWarps) * kTile;
+      const int j0 = (tile0 + warp + i * W) * kTile;
       unsigned char* sk = ring + st * R::kStageBytes;
       unsigned char* sv = sk + R::kTileBytes;
       const bool in = j0 + lane < n, fine = page_ok(a.view, page);
@@ -446,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
     next_page = page_of(i + kStages);
     cp_async_wait<kStages - 1>();
     __syncwarp();
-    const int j0 = (tile0 + warp + i * kWarps) * kTile;
+    const int j0 = (tile0 + warp + i * W) * kTile;
     const unsigned char* sk = ring + st * R::kStageBytes;
     const unsigned char* sv = sk + R::kTileBytes;
     const float* ss = reinterpret_cast<const float*>(sv + R::kTileBytes);
@@ -637,10 +645,10 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
   }
   __syncthreads();  // s_bad is initialised and every ring is idle: the rings hold the join
   if (__any_sync(0xffffffffu, bad) && lane == 0) s_bad = 1;
-  using J = Join<D, NH>;
+  using J = Join<D, NH, W>;
   float* red_o = reinterpret_cast<float*>(smem);
-  float* red_ml = red_o + kWarps * J::kHeads * J::kRedRow;
-  float* cta_o = red_ml + kWarps * J::kHeads * 2;  // [heads][D]
+  float* red_ml = red_o + W * J::kHeads * J::kRedRow;
+  float* cta_o = red_ml + W * J::kHeads * 2;  // [heads][D]
   float* cta_ml = cta_o + J::kHeads * D;           // [heads][4]: max, sum, the bad mark
   const float back = I8 ? vref : 1.f;
 #pragma unroll
@@ -684,11 +692,11 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
   };
   for (int quad = threadIdx.x; quad < G * D / 4; quad += kThreads) {
     const int head = quad / (D / 4), d = quad % (D / 4) * 4;
-    float2 ml[kWarps];
-    float4 x[kWarps];
+    float2 ml[W];
+    float4 x[W];
     float M = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       ml[w] = *reinterpret_cast<const float2*>(red_ml + (w * J::kHeads + head) * 2);
       x[w] = *reinterpret_cast<const float4*>(red_o + (w * J::kHeads + head) * J::kRedRow + d);
       M = fmaxf(M, ml[w].x);
@@ -696,7 +704,7 @@ __global__ void __launch_bounds__(kThreads, min_ctas(D, I8, NH)) attn_paged_kern
     float L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float f = join_weight(ml[w].x, M);  // a warp without tiles holds zeros and weight 0
       L = fmaf(f, ml[w].y, L);
       fma4(acc, f, x[w]);
@@ -887,6 +895,20 @@ int check_heads(const char* what, int64_t n_tokens, int64_t n_heads, int64_t hkv
   return KLLM_B200_OK;
 }
 
+// Narrow: many short items are bound by a CTA's fixed 3 to 5 us (dependent first
+// loads, the join), so there a CTA is one warp, with a quarter of the shared
+// memory and more than twice to seven times the CTAs per SM. By waves of the
+// four-warp form: the longer the sequences may be, the more waves it takes
+// until the device stays full to the end without several warps per item.
+// Measured, us, four warps / one, lengths of a quarter to all of the capacity:
+//                          capacity 32      128         512         1024        2048
+//   fp16 14/2 x 64    2000 items 14 / 8     17 / 11     32 / 33     55 / 59     100 / 109
+//                    16000      109 / 39   121 / 61    215 / 198   383 / 383    741 / 750
+//   fp16 32/32 x 128  1984       35 / 9     42 / 18     70 / 52    111 / 100    192 / 192
+//                    16000      298 / 58   314 / 102   535 / 361   832 / 715   1514 / 1421
+//   int8 32/32 x 128  1984       25 / 17    27 / 22     44 / 41     64 / 73     107 / 128
+//                    16000      163 / 91   186 / 128   304 / 235   440 / 398    766 / 779
+//
 // How the positions of a (token, kv head) are dealt out, by sizes the host
 // knows: the largest cluster of which the device holds one for every item at
 // once, and, where the largest leaves room, several clusters per item while a
@@ -899,15 +921,16 @@ int check_heads(const char* what, int64_t n_tokens, int64_t n_heads, int64_t hkv
 //   fp16 128 sequences  31.1 / 30.6 / 31.5 / 46.0;  512: 87.4 / 88.0 / 100  / 166
 struct Split {
   int cluster, splits;
-  bool order;
+  bool order, narrow;
 };
 
 template <int D, bool I8, int NH>
 Split split_of(int64_t n_tokens, int64_t hkv, int64_t capacity) {
   const int64_t items = n_tokens * hkv;
-  const void* kernel = reinterpret_cast<const void*>(attn_paged_kernel<D, I8, NH>);
-  const size_t smem = Ring<D, I8>::kBytes;
-  Split x = {1, 1, false};
+  const void* kernel = reinterpret_cast<const void*>(attn_paged_kernel<D, I8, NH, kWarps>);
+  constexpr int kThreads = kWarps * 32;
+  constexpr size_t smem = smem_bytes<D, I8, NH, kWarps>();
+  Split x = {1, 1, false, false};
   (void)allow_smem(kernel, smem);  // occupancy is asked for with the opt-in in place
   for (int c = kMaxCluster; c > 1; c /= 2) {
     if (capacity < c * kWarps * kTile) continue;
@@ -924,6 +947,7 @@ Split split_of(int64_t n_tokens, int64_t hkv, int64_t capacity) {
   const int64_t slots = static_cast<int64_t>(sm_count()) * resident_ctas_raw(kernel, kThreads, smem);
   x.order = x.cluster == 1 && items > slots && items <= kOrderWaves * slots && n_tokens > 1 &&
             n_tokens <= kOrderThreads * kOrderPer && capacity >= KLLM_B200_PAGED_SPLIT_MIN;
+  x.narrow = x.cluster == 1 && items > slots && items * kNarrow >= capacity * slots;
   return x;
 }
 
@@ -941,12 +965,12 @@ int64_t workspace_for(int64_t n_tokens, int64_t n_heads, int64_t head_dim, const
   return split.splits <= 1 ? 0 : n_tokens * n_heads * split.splits * (head_dim + 2) * static_cast<int64_t>(sizeof(float));
 }
 
-template <int D, bool I8, int NH>
+template <int D, bool I8, int NH, int W>
 int launch_attention(const PagedAttnArgs& a, const LaunchOpts& o) {
   const char* what = "attention_paged";
-  const size_t smem = Ring<D, I8>::kBytes;
-  static_assert(Ring<D, I8>::kBytes >= Join<D, NH>::kBytes, "the join fits the rings");
-  auto kernel = attn_paged_kernel<D, I8, NH>;
+  constexpr int kThreads = W * 32;
+  constexpr size_t smem = smem_bytes<D, I8, NH, W>();
+  auto kernel = attn_paged_kernel<D, I8, NH, W>;
   cudaError_t err = allow_smem(reinterpret_cast<const void*>(kernel), smem);
   if (err != cudaSuccess) return launch_status(err, "attention_paged: shared memory opt-in");
   const dim3 grid(static_cast<unsigned>(a.n_tokens * a.view.n_kv_heads * a.splits * a.cluster));
@@ -964,8 +988,9 @@ int launch_attention(const PagedAttnArgs& a, const LaunchOpts& o) {
 }
 
 template <int D, bool I8>
-int launch_groups(const PagedAttnArgs& a, const LaunchOpts& o) {
-  return a.groups <= 8 ? launch_attention<D, I8, 1>(a, o) : launch_attention<D, I8, 2>(a, o);
+int launch_groups(const PagedAttnArgs& a, bool narrow, const LaunchOpts& o) {
+  if (narrow) return a.groups <= 8 ? launch_attention<D, I8, 1, 1>(a, o) : launch_attention<D, I8, 2, 1>(a, o);
+  return a.groups <= 8 ? launch_attention<D, I8, 1, kWarps>(a, o) : launch_attention<D, I8, 2, kWarps>(a, o);
 }
 
 }  // namespace
@@ -1033,8 +1058,8 @@ int attention_paged(const void* q, int64_t q_stride, const kllm_b200_paged_cache
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + n_tokens * n_heads * split.splits * D;
   }
-  if (cache->cache_dtype == KLLM_B200_I8) return D == 64 ? launch_groups<64, true>(a, o) : launch_groups<128, true>(a, o);
-  return D == 64 ? launch_groups<64, false>(a, o) : launch_groups<128, false>(a, o);
+  if (cache->cache_dtype == KLLM_B200_I8) return D == 64 ? launch_groups<64, true>(a, split.narrow, o) : launch_groups<128, true>(a, split.narrow, o);
+  return D == 64 ? launch_groups<64, false>(a, split.narrow, o) : launch_groups<128, false>(a, split.narrow, o);
 }
 
 }  // namespace kb

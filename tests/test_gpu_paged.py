@@ -775,6 +775,51 @@ def test_attention_longest_first(cuda, ops, dtype, hkv, d, n, longest):
             assert ((got[t] - want).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d,n,longest", [
+    (14, 2, 64, 600, 128),     # Qwen2.5-0.5B heads
+    (32, 32, 128, 40, 33),     # Llama-2-7B heads, one position past a tile
+    (16, 1, 64, 1000, 64),     # two tiles of heads
+    (32, 2, 128, 700, 100),
+    (9, 3, 128, 500, 1),
+    (4, 2, 64, 3001, 500),
+])
+def test_attention_many_short(cuda, ops, dtype, hq, hkv, d, n, longest):
+    """Batches of many short items (a CTA of one warp each), ragged, with
+    padding and a bad page; sequences share pages."""
+    rng = np.random.default_rng(hq + n)
+    page, n_pages = 8, 50
+    max_pages = -(-longest // page)
+    table = rng.integers(0, n_pages, (n, max_pages)).astype(np.int32)
+    cache, k, v = pu.random_cache(rng, ops, dtype, n_pages, hkv, page, d, table)
+    positions = rng.integers(0, longest, n)
+    positions[rng.integers(0, n, 2)] = longest - 1
+    seqs = rng.permutation(n)
+    q = randh(rng, n, hq, d, scale=1.5).cuda()
+    assert ops.attention_paged_workspace_bytes(n, hq, cache) == 0
+    err = flags()
+    out = ops.attention_paged(q, cache, i32(positions), i32(seqs), err_flags=err)
+    torch.cuda.synchronize()
+    assert int(err.item()) == 0
+    got = out.cpu().double()
+    for t in rng.permutation(n)[:20].tolist() + [int(positions.argmax()), int(positions.argmin())]:
+        p, at = int(positions[t]), int(seqs[t])
+        want, bound = pu.attention(q[t].cpu().double(), pu.rows_of(k, table, at, p + 1), pu.rows_of(v, table, at, p + 1))
+        assert ((got[t] - want).abs() <= bound).all()
+    # padding and a page out of range: zeros there, no bit elsewhere changes
+    from littlellm_b200 import _capi
+    positions[7] = -1
+    bad = table.copy()
+    bad[seqs[11], int(positions[11]) // page] = n_pages
+    cache.page_table.copy_(torch.from_numpy(bad))
+    again = ops.attention_paged(q, cache, i32(positions), i32(seqs), err_flags=err)
+    torch.cuda.synchronize()
+    assert int(err.item()) == _capi.FLAG_BAD_PAGE
+    assert bool((again[[7, 11]] == 0).all())
+    rest = [t for t in range(n) if t not in (7, 11)]
+    assert torch.equal(again[rest], out[rest])
+
+
 def test_attention_longest_first_in_a_graph(cuda, ops):
     """The order is made from the positions of each replay; lengths all equal,
     ragged, and all padding."""
