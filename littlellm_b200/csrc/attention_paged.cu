@@ -400,6 +400,11 @@ __global__ void __launch_bounds__(W * 32, min_ctas(D, I8, NH, W)) attn_paged_ker
 #pragma unroll
     for (int i = 0; i < kQuads; ++i) {
       const int quad = threadIdx.x + i * kThreads;  // D / 4 lanes of a warp hold a head
+      if (4 * (warp * 32 + i * kThreads) >= G * D) {  // no head in this warp's: one head per kv head leaves 7 of 8 out
+        for (int d = 0; d < 3; ++d) s_digits[d][quad] = 0u;
+        if (quad % (D / 4) == 0) s_unit[quad / (D / 4)] = 0.f;
+        continue;
+      }
       const float2 x = h2_to_f2(raw[i].x), y = h2_to_f2(raw[i].y);
       float qmax = max_nan(max_nan(fabsf(x.x), fabsf(x.y)), max_nan(fabsf(y.x), fabsf(y.y)));
 #pragma unroll
