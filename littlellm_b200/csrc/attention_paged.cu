@@ -67,6 +67,9 @@ constexpr int kCombineWarps = 4;
 constexpr int kOrderThreads = 1024, kOrderPer = 8;  // tokens that one CTA puts in order: 8192
 constexpr int kOrderWaves = 8;    // a batch of more waves of CTAs is not put in order,
 constexpr int kLong = 2048;       // nor one without a sequence of this many positions
+constexpr int kPartWaves = 4;     // waves of CTAs up to which long sequences are split,
+constexpr int64_t kPart = 4096;   // positions of capacity that a CTA keeps at least then,
+constexpr int kPartLeast = 1024;  // and of a sequence
 constexpr int64_t kNarrow = 128;  // positions of capacity per wave of CTAs up to which a CTA is one warp
 constexpr float kLift = 11.f;    // log2 of the power of a score at the reference
 constexpr float kMost = 32768.f;  // a larger power moves the reference (fp16 ends at 65504)
@@ -88,12 +91,21 @@ struct PagedAttnArgs {
   int cluster;     // CTAs per cluster
   int splits;      // clusters per (token, kv head)
   int parts_shift;  // log2(cluster * splits)
+  int min_tiles;   // tiles of a CTA below which a sequence takes fewer clusters
   float* part_o;   // [T, Hq, splits, D], sums of p v against the part's own max
   float* part_ml;  // [T, Hq, splits, 2] (max, sum); sum -1: the part met a bad page
   int4* order;     // [T] (token, position, sequence, -), longest first, or NULL
   int32_t* err_flags;
   float scale_log2;  // log2(e) / sqrt(D)
 };
+
+// Tiles of each CTA of a sequence of all_tiles: the clusters that have
+// min_tiles for each of their CTAs (one at least) share them.
+__device__ __forceinline__ int tiles_per_part(const PagedAttnArgs& a, int all_tiles) {
+  const int least = a.cluster * a.min_tiles;
+  const int clusters = max(1, min(a.splits, (all_tiles + least - 1) / least));
+  return (all_tiles + clusters * a.cluster - 1) / (clusters * a.cluster);
+}
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int src_bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
@@ -309,7 +321,7 @@ __global__ void __launch_bounds__(W * 32, min_ctas(D, I8, NH, W)) attn_paged_ker
   }
   const int n = pos + 1;
   const int all_tiles = (n + kTile - 1) / kTile;
-  const int per_part = (all_tiles + parts - 1) / parts;
+  const int per_part = tiles_per_part(a, all_tiles);
   const int cluster_part = part / a.cluster;
   if (cluster_part * a.cluster * per_part >= all_tiles) return;  // nothing left for this cluster
   const int tile0 = min(part * per_part, all_tiles);
@@ -766,8 +778,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attn_paged_combine_kernel(
     int flag;
     if (token_state(a.view, pos, seq, flag) == kTokenOk) {
       const int all_tiles = (pos + kTile) / kTile;
-      const int parts = a.splits * a.cluster;
-      const int per_cluster = (all_tiles + parts - 1) / parts * a.cluster;
+      const int per_cluster = tiles_per_part(a, all_tiles) * a.cluster;
       used = (all_tiles + per_cluster - 1) / per_cluster;
     }
   }
@@ -900,6 +911,15 @@ int check_heads(const char* what, int64_t n_tokens, int64_t n_heads, int64_t hkv
   return KLLM_B200_OK;
 }
 
+// Batches of one wave at most over long caches are split further than fits at
+// once, while a CTA keeps kPart positions of the capacity: padded rows and short
+// sequences then leave no slot idle, and the longest ones are shared. A sequence
+// takes the clusters that have kPartLeast positions for each of their CTAs.
+// Measured, us, without / with: int8, 40/8 x 128, 2 sequences of 51 and 91
+// thousand and 5 padded rows 147 / 61; 6/6 x 64, 4 of 63 to 100 thousand and 5
+// padded rows 79 / 55; 16/1 x 64, 94 of 51 to 67 thousand 245 / 190; 14/2 x 64,
+// 64 of 100 to 32768 79 / 70; fp16, 14/2 x 64, 64 of 32768 each 158 / 163.
+//
 // Narrow: many short items are bound by a CTA's fixed 3 to 5 us (dependent first
 // loads, the join), so there a CTA is one warp, with a quarter of the shared
 // memory and more than twice to seven times the CTAs per SM. By waves of the
@@ -927,6 +947,7 @@ int check_heads(const char* what, int64_t n_tokens, int64_t n_heads, int64_t hkv
 struct Split {
   int cluster, splits;
   bool order, narrow;
+  int min_tiles;
 };
 
 template <int D, bool I8, int NH>
@@ -935,7 +956,7 @@ Split split_of(int64_t n_tokens, int64_t hkv, int64_t capacity) {
   const void* kernel = reinterpret_cast<const void*>(attn_paged_kernel<D, I8, NH, kWarps>);
   constexpr int kThreads = kWarps * 32;
   constexpr size_t smem = smem_bytes<D, I8, NH, kWarps>();
-  Split x = {1, 1, false, false};
+  Split x = {1, 1, false, false, 1};
   (void)allow_smem(kernel, smem);  // occupancy is asked for with the opt-in in place
   for (int c = kMaxCluster; c > 1; c /= 2) {
     if (capacity < c * kWarps * kTile) continue;
@@ -950,9 +971,14 @@ Split split_of(int64_t n_tokens, int64_t hkv, int64_t capacity) {
   }
   // more than one wave, few enough that its last one counts
   const int64_t slots = static_cast<int64_t>(sm_count()) * resident_ctas_raw(kernel, kThreads, smem);
-  x.order = x.cluster == 1 && items > slots && items <= kOrderWaves * slots && n_tokens > 1 &&
+  while (items <= slots && x.splits < kMaxSplits && items * x.cluster * x.splits * 2 <= kPartWaves * slots &&
+         capacity >= 2 * kPart * x.cluster * x.splits) {
+    x.splits *= 2;
+    x.min_tiles = kPartLeast / kTile;
+  }
+  x.order = x.cluster == 1 && x.splits == 1 && items > slots && items <= kOrderWaves * slots && n_tokens > 1 &&
             n_tokens <= kOrderThreads * kOrderPer && capacity >= KLLM_B200_PAGED_SPLIT_MIN;
-  x.narrow = x.cluster == 1 && items > slots && items * kNarrow >= capacity * slots;
+  x.narrow = x.cluster == 1 && x.splits == 1 && items > slots && items * kNarrow >= capacity * slots;
   return x;
 }
 
@@ -1055,6 +1081,7 @@ int attention_paged(const void* q, int64_t q_stride, const kllm_b200_paged_cache
   a.groups = static_cast<int>(n_heads / a.view.n_kv_heads);
   a.cluster = split.cluster;
   a.splits = split.splits;
+  a.min_tiles = split.min_tiles;
   while ((1 << a.parts_shift) < a.cluster * a.splits) ++a.parts_shift;
   a.err_flags = err_flags;
   a.scale_log2 = 1.4426950408889634f / sqrtf(static_cast<float>(D));

@@ -776,6 +776,40 @@ def test_attention_longest_first(cuda, ops, dtype, hkv, d, n, longest):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,d,n", [(14, 2, 64, 60), (4, 4, 128, 36), (16, 1, 64, 90), (5, 1, 128, 9)])
+def test_attention_long_and_padded(cuda, ops, dtype, hq, hkv, d, n):
+    """Padded batches over a long cache, split into more parts than run at
+    once; sequences share pages, lengths from one position to all."""
+    rng = np.random.default_rng(hq + n)
+    page, n_pages, capacity = 64, 96, 65536
+    table = rng.integers(0, n_pages, (n, capacity // page)).astype(np.int32)
+    cache, k, v = pu.random_cache(rng, ops, dtype, n_pages, hkv, page, d, table)
+    lengths = [1, 32, 33, 1023, 1024, 1025, 4097, 40_000, 65_536]
+    positions = np.full(n, -1)
+    at = rng.permutation(n)[:len(lengths)]
+    positions[at] = np.array(lengths) - 1
+    seqs = rng.permutation(n)
+    q = randh(rng, n, hq, d, scale=1.5).cuda()
+    nbytes = ops.attention_paged_workspace_bytes(n, hq, cache)
+    assert nbytes > 0 and nbytes % (n * hq * (d + 2) * 4) == 0
+    ws = torch.full((nbytes + 64,), 0x7f, dtype=torch.uint8, device="cuda")
+    for work in (ws[:nbytes], ws[:nbytes // 2], ws[:0]):
+        check = np.concatenate([at, np.flatnonzero(positions == -1)])
+        out = check_attention(ops, q, cache, (k, v), table, positions.tolist(), seqs.tolist(), workspace=work) \
+            if work.numel() == nbytes else ops.attention_paged(q, cache, i32(positions), i32(seqs), workspace=work)
+        if work.numel() == nbytes:
+            again = ops.attention_paged(q, cache, i32(positions), i32(seqs), workspace=work)
+            assert torch.equal(out, again)
+        else:  # two forms of one answer, each within the bound checked above of the same value
+            want = [pu.attention(q[t].cpu().double(), pu.rows_of(k, table, int(seqs[t]), int(positions[t]) + 1),
+                                 pu.rows_of(v, table, int(seqs[t]), int(positions[t]) + 1)) for t in at[:6]]
+            for t, (w, bound) in zip(at[:6], want):
+                assert ((out[t].cpu().double() - w).abs() <= bound).all()
+            assert bool((out[check[len(at):]] == 0).all())
+    assert bool((ws[nbytes:] == 0x7f).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("hq,hkv,d,n,longest", [
     (14, 2, 64, 600, 128),     # Qwen2.5-0.5B heads
     (32, 32, 128, 40, 33),     # Llama-2-7B heads, one position past a tile
