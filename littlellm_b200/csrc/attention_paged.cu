@@ -8,7 +8,8 @@
 // (token, kv head), and is bound by HBM.
 //
 // The positions of a (token, kv head) are dealt to the CTAs of a cluster (and,
-// for few tokens over a long cache, to several clusters). A CTA's four warps
+// for few tokens over a long cache, to several clusters). A CTA's four warps (one,
+// where there are many short items)
 // stream 32-position tiles of K and V through a per-warp cp.async ring, the
 // rows' addresses taken from the page table one tile ahead; pages hold eight
 // positions at least, so eight rows share one address. Both products run on
@@ -266,7 +267,8 @@ constexpr size_t smem_bytes() {
 }
 
 template <int D, bool I8, int NH, int W>
-__global__ void __launch_bounds__(W * 32, min_ctas(D, I8, NH, W)) attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
+__global__ void __launch_bounds__(W * 32, min_ctas(D, I8, NH, W))
+attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
   using R = Ring<D, I8, W>;
   constexpr int kThreads = W * 32;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -280,7 +282,8 @@ __global__ void __launch_bounds__(W * 32, min_ctas(D, I8, NH, W)) attn_paged_ker
   const int parts = 1 << a.parts_shift;  // clusters and splits are powers of two
   const unsigned item = blockIdx.x >> a.parts_shift, hkv = a.view.n_kv_heads;
   const int part = blockIdx.x & (parts - 1);
-  const unsigned place = item / hkv;  // a token's heads side by side, neighbours in its pages (90 against 94 us at 29 x 32 heads)
+  // a token's heads side by side, neighbours in its pages (90 against 94 us at 29 x 32 heads)
+  const unsigned place = item / hkv;
   const int g = static_cast<int>(item - place * hkv);
   const int G = a.groups;
   if (threadIdx.x == 0) s_bad = 0;
@@ -651,7 +654,7 @@ __global__ void __launch_bounds__(W * 32, min_ctas(D, I8, NH, W)) attn_paged_ker
   }
   cp_async_wait<0>();
 
-  // join the four warps; a head's sum is spread over the eight lanes of its column
+  // join the warps; a head's sum is spread over the eight lanes of its column
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
 #pragma unroll
@@ -822,7 +825,9 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attn_paged_combine_kernel(
 
 // Class of a length >= 1, longest first: eighths of octaves, by the top bits of
 // its float (exponent and three bits, 1016 for 1).
-__host__ __device__ constexpr int length_class(uint32_t float_bits) { return 255 - (static_cast<int>(float_bits >> 20) - 1016); }
+__host__ __device__ constexpr int length_class(uint32_t float_bits) {
+  return 255 - (static_cast<int>(float_bits >> 20) - 1016);
+}
 
 // Tokens, longest first, for grids of more CTAs than run at once: CTAs start in
 // the order of their index, so the last ones to start are the shortest and the
@@ -986,8 +991,11 @@ Split preferred_split(int64_t n_tokens, int64_t n_heads, const PagedView& view, 
   const auto pick = [&](auto narrow, auto wide) {
     return (n_heads / view.n_kv_heads <= 8 ? narrow : wide)(n_tokens, view.n_kv_heads, view.capacity);
   };
-  if (head_dim == 64) return i8 ? pick(split_of<64, true, 1>, split_of<64, true, 2>) : pick(split_of<64, false, 1>, split_of<64, false, 2>);
-  return i8 ? pick(split_of<128, true, 1>, split_of<128, true, 2>) : pick(split_of<128, false, 1>, split_of<128, false, 2>);
+  if (head_dim == 64) {
+    return i8 ? pick(split_of<64, true, 1>, split_of<64, true, 2>) : pick(split_of<64, false, 1>, split_of<64, false, 2>);
+  }
+  return i8 ? pick(split_of<128, true, 1>, split_of<128, true, 2>)
+            : pick(split_of<128, false, 1>, split_of<128, false, 2>);
 }
 
 // The workspace: parts to join, or the order of the tokens; never both.
@@ -1090,7 +1098,9 @@ int attention_paged(const void* q, int64_t q_stride, const kllm_b200_paged_cache
     a.part_o = static_cast<float*>(workspace);
     a.part_ml = a.part_o + n_tokens * n_heads * split.splits * D;
   }
-  if (cache->cache_dtype == KLLM_B200_I8) return D == 64 ? launch_groups<64, true>(a, split.narrow, o) : launch_groups<128, true>(a, split.narrow, o);
+  if (cache->cache_dtype == KLLM_B200_I8) {
+    return D == 64 ? launch_groups<64, true>(a, split.narrow, o) : launch_groups<128, true>(a, split.narrow, o);
+  }
   return D == 64 ? launch_groups<64, false>(a, split.narrow, o) : launch_groups<128, false>(a, split.narrow, o);
 }
 
