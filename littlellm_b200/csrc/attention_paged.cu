@@ -29,14 +29,20 @@
 // probabilities. (K through the same conversion was 2 to 3% slower at 2048
 // sequences of up to 4095 positions, where instruction issue is the bound.)
 //
-// Softmax: each warp keeps a reference m per head and takes the powers
-// 2^(s - m + kLift). Only a tile with a power above kMost (in practice the
-// first one) pays for a new maximum, a rescale of the sums and its powers
-// again. kLift places the largest probabilities near the top of
-// fp16's range, so that those down to 2^-25 of the largest keep 11 bits as
-// operands of the second product; for int8 rows, whose probabilities carry the
-// scale of the value, that scale is taken relative to a power of two at or
-// above the largest the warp has met. Scores, sums and accumulators are fp32.
+// Softmax: each warp keeps a reference r per head and takes the powers
+// 2^(s - r). Only a tile with a power above kMost (in practice the first one)
+// pays for a new reference, a rescale of the sums and its powers again. r lies
+// kLift below the largest score met, which places the largest probabilities
+// near the top of fp16's range, so that those down to 2^-25 of the largest keep
+// 11 bits as operands of the second product; for int8 rows, whose probabilities
+// carry the scale of the value, that scale is taken relative to a power of two
+// at or above the largest the warp has met. Scores, sums and accumulators are
+// fp32. Rescales and joins go by r itself, rounded as the powers saw it: the
+// maximum in its place would misweigh the parts by its rounding, two percent at
+// scores of 2^19. While the largest score is below kFar, an exponent is one FMA:
+// the dot product times its factor, exact, minus r. Past that the product is
+// rounded first, as it is for the maximum: what that rounding leaves out (half a
+// step, 16 at 2^28) would take the largest power out of fp16's range.
 //
 // Batches of more items than run at once are taken longest first.
 //
@@ -72,8 +78,10 @@ constexpr int kPartWaves = 4;     // waves of CTAs up to which long sequences ar
 constexpr int64_t kPart = 4096;   // positions of capacity that a CTA keeps at least then,
 constexpr int kPartLeast = 1024;  // and of a sequence
 constexpr int64_t kNarrow = 128;  // positions of capacity per wave of CTAs up to which a CTA is one warp
-constexpr float kLift = 11.f;    // log2 of the power of a score at the reference
-constexpr float kMost = 32768.f;  // a larger power moves the reference (fp16 ends at 65504)
+constexpr float kLift = 11.f;      // log2 of the power of the score that sets the reference
+constexpr float kMost = 32768.f;   // a larger power moves the reference (fp16 ends at 65504)
+constexpr float kFar = 0x1p20f;    // scores (log2 units) from which products are rounded before the reference is taken
+constexpr float kUnset = -3.4028235e38f;  // reference of a head that has met no score: every power is infinite
 
 struct PagedAttnArgs {
   const __half* q;
@@ -93,8 +101,8 @@ struct PagedAttnArgs {
   int splits;      // clusters per (token, kv head)
   int parts_shift;  // log2(cluster * splits)
   int min_tiles;   // tiles of a CTA below which a sequence takes fewer clusters
-  float* part_o;   // [T, Hq, splits, D], sums of p v against the part's own max
-  float* part_ml;  // [T, Hq, splits, 2] (max, sum); sum -1: the part met a bad page
+  float* part_o;   // [T, Hq, splits, D], sums of p v against the part's own reference
+  float* part_ml;  // [T, Hq, splits, 2] (reference, sum); sum -1: the part met a bad page
   int4* order;     // [T] (token, position, sequence, -), longest first, or NULL
   int32_t* err_flags;
   float scale_log2;  // log2(e) / sqrt(D)
@@ -250,9 +258,16 @@ struct Join {
   static constexpr int kBytes = (W * kHeads * (kRedRow + 2) + kHeads * (D + 4)) * 4;
 };
 
-// One row's (or part's) share of the joined output: exp2 of its max against the
-// joint max; a part that saw nothing has max -inf and weight 0.
-__device__ __forceinline__ float join_weight(float m, float top) { return m == -INFINITY ? 0.f : exp2_approx(m - top); }
+// Reference for a largest score x: kLift below it where fp32 has such a number
+// to a unit, else the nearest below that it has, or x itself (steps of 16 and
+// more; an infinity). The power of x is then at most 2^(kLift + 1).
+__device__ __forceinline__ float reference_of(float x) {
+  const float r = x - kLift;
+  return x - r <= kLift + 1.f ? r : x;
+}
+// One row's (or part's) share of the joined output: exp2 of its reference against
+// the joint one; a part that saw nothing (kUnset) has weight 0 beside any other.
+__device__ __forceinline__ float join_weight(float r, float top) { return exp2_approx(r - top); }
 
 // Resident CTAs that the registers are held to: int8 rows of 64 codes have the
 // shared memory for five, and want their warps (2048 sequences of up to 4095
@@ -454,13 +469,13 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
   }
 
   float o[NH][kM][4];
-  // m: the heads' references; at = kLift - m. Before the first tile every power
-  // is infinite, which makes that tile set them.
-  float m[NH][2], at[NH][2], l[NH][2];
+  // ref: the heads' references. Before the first tile every power is infinite,
+  // which makes that tile set them.
+  float ref[NH][2], l[NH][2];
+  bool far = false;  // some head of the warp has met a score of kFar
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
-    m[h][0] = m[h][1] = -INFINITY;
-    at[h][0] = at[h][1] = 3.4028235e38f;
+    ref[h][0] = ref[h][1] = kUnset;
     l[h][0] = l[h][1] = 0.f;
 #pragma unroll
     for (int i = 0; i < kM; ++i) o[h][i][0] = o[h][i][1] = o[h][i][2] = o[h][i][3] = 0.f;
@@ -529,13 +544,26 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
     }
     float p[2][NH][4];
     const bool last = j0 + kTile > n;
+    // the scores as rounded products
+    auto round_scores = [&]() {
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[mt][h][e] = __fmul_rn(s[mt][h][e], f[mt][e >> 1]);
+        }
+        f[mt][0] = f[mt][1] = 1.f;
+      }
+    };
+    if (far) round_scores();
     auto powers = [&]() {
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
         for (int h = 0; h < NH; ++h) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) p[mt][h][e] = exp2_approx(fmaf(s[mt][h][e], f[mt][e >> 1], at[h][e & 1]));
+          for (int e = 0; e < 4; ++e) p[mt][h][e] = exp2_approx(fmaf(s[mt][h][e], f[mt][e >> 1], -ref[h][e & 1]));
         }
       }
       if (last) {
@@ -577,25 +605,39 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
           inv_vref = 1.f / up;
         }
       }
+      float top[NH][2];
+      bool high = false;
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
-        float cr[2];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float x = m[h][e];
+          float x = -INFINITY;
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
-              if (j0 + mt * 16 + gid + 8 * half < n) x = fmaxf(x, s[mt][h][2 * half + e] * f[mt][half]);
+              if (j0 + mt * 16 + gid + 8 * half < n) x = fmaxf(x, __fmul_rn(s[mt][h][2 * half + e], f[mt][half]));
             }
           }
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-          cr[e] = m[h][e] == -INFINITY ? 0.f : exp2_approx(m[h][e] - x);
-          m[h][e] = x;
-          if (x != -INFINITY) at[h][e] = kLift - x;  // all scores -inf so far: still unset
+          top[h][e] = x;
+          high |= fabsf(x) >= kFar && x != -INFINITY;
+        }
+      }
+      if (!far && __any_sync(0xffffffffu, high)) {
+        far = true;
+        round_scores();
+      }
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        float cr[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float r = fmaxf(ref[h][e], reference_of(top[h][e]));  // all scores -inf so far: still unset
+          cr[e] = exp2_approx(ref[h][e] - r);
+          ref[h][e] = r;
           l[h][e] *= cr[e];
           cr[e] *= ratio;
         }
@@ -669,7 +711,7 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
   float* red_o = reinterpret_cast<float*>(smem);
   float* red_ml = red_o + W * J::kHeads * J::kRedRow;
   float* cta_o = red_ml + W * J::kHeads * 2;  // [heads][D]
-  float* cta_ml = cta_o + J::kHeads * D;           // [heads][4]: max, sum, the bad mark
+  float* cta_ml = cta_o + J::kHeads * D;           // [heads][4]: reference, sum, the bad mark
   const float back = I8 ? vref : 1.f;
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
@@ -685,7 +727,7 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
     if (gid == 0) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        red_ml[(warp * J::kHeads + h * 8 + 2 * tig + e) * 2] = m[h][e];
+        red_ml[(warp * J::kHeads + h * 8 + 2 * tig + e) * 2] = ref[h][e];
         red_ml[(warp * J::kHeads + h * 8 + 2 * tig + e) * 2 + 1] = l[h][e];
       }
     }
@@ -714,7 +756,7 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
     const int head = quad / (D / 4), d = quad % (D / 4) * 4;
     float2 ml[W];
     float4 x[W];
-    float M = -INFINITY;
+    float M = kUnset;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
       ml[w] = *reinterpret_cast<const float2*>(red_ml + (w * J::kHeads + head) * 2);
@@ -744,10 +786,10 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
     float4 ml[kMaxCluster], x[kMaxCluster];
 #pragma unroll
     for (int c = 0; c < kMaxCluster; ++c) {
-      ml[c] = c < a.cluster ? ld_peer(cta_ml + 4 * head, c) : make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      ml[c] = c < a.cluster ? ld_peer(cta_ml + 4 * head, c) : make_float4(kUnset, 0.f, 0.f, 0.f);
       x[c] = c < a.cluster ? ld_peer(cta_o + head * D + d, c) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
-    float M = -INFINITY, L = 0.f;
+    float M = kUnset, L = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int c = 0; c < kMaxCluster; ++c) {
@@ -788,10 +830,10 @@ __global__ void __launch_bounds__(kCombineWarps * 32) attn_paged_combine_kernel(
   grid_dep_wait();
   grid_dep_launch();
   if (used <= 1) return;  // written by the attention kernel
-  // lane c holds part c's max and sum; its weight goes to all by shuffles
+  // lane c holds part c's reference and sum; its weight goes to all by shuffles
   const float* ml = a.part_ml + row * a.splits * 2;
   const float* po = a.part_o + row * a.splits * D + lane * kPer;
-  float pm = -INFINITY, pl = 0.f;
+  float pm = kUnset, pl = 0.f;
   if (lane < used) {
     pm = ml[2 * lane];
     pl = ml[2 * lane + 1];
