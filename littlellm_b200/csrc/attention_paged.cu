@@ -37,12 +37,11 @@
 // 11 bits as operands of the second product; for int8 rows, whose probabilities
 // carry the scale of the value, that scale is taken relative to a power of two
 // at or above the largest the warp has met. Scores, sums and accumulators are
-// fp32. Rescales and joins go by r itself, rounded as the powers saw it: the
-// maximum in its place would misweigh the parts by its rounding, two percent at
-// scores of 2^19. While the largest score is below kFar, an exponent is one FMA:
-// the dot product times its factor, exact, minus r. Past that the product is
-// rounded first, as it is for the maximum: what that rounding leaves out (half a
-// step, 16 at 2^28) would take the largest power out of fp16's range.
+// fp32. Rescales and joins go by r itself: past 2^24 kLift no longer comes off
+// the maximum exactly. While the largest score is below kFar, an exponent is one
+// FMA: the dot product times its factor, exact, minus r. Past that the product
+// is rounded first, as it is for the maximum: what that rounding leaves out
+// (half a step, 16 at 2^28) would take the largest power out of fp16's range.
 //
 // Batches of more items than run at once are taken longest first.
 //
