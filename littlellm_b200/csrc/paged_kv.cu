@@ -94,12 +94,16 @@ __device__ __forceinline__ float max_nan(float a, float b) {
   return r;
 }
 
-// rint(x / scale) of 16 values as 16 codes. inv is 1 / scale to an ulp or two,
-// so q = x * inv is off by a few steps of fp32; one residual step
-// (q += (x - q scale) inv, as in division by a reciprocal) gives the quotient
-// rounded, so a value half way between two codes is seen as such and goes to
-// the even one. Adding 1.5 * 2^23 rounds to a whole number, ties to even, and
-// leaves the code in the low byte.
+// rint(x / scale) of eight values as codes, the quotient by Markstein's residual
+// correction (P. Markstein, Computation of elementary functions on the IBM RISC
+// System/6000 processor, 1990). inv is 1 / scale to an ulp or two, so q = x inv
+// is off by some 2^-22; r = x - q scale is exact as an FMA but for a rounding,
+// and q + r inv is off by that error's square, 2^-45, before it is rounded. So a
+// value half way between two codes is seen as such and goes to the even one, and
+// codes are those of the fp32 quotient (all pairs of fp16 significands, and three
+// million fp32 values within two steps of half way, agree bit for bit). Adding
+// 1.5 * 2^23 rounds to a whole number, ties to even, and leaves the code in the
+// low byte.
 __device__ __forceinline__ uint2 codes8(const float (&x)[8], float scale, float inv) {
   const unsigned long long i2 = f32x2_pack(inv, inv), n2 = f32x2_pack(-scale, -scale);
   const unsigned long long magic = f32x2_pack(12582912.f, 12582912.f);
@@ -274,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, SHARED && U > 1 ? (I8 ? 9 : 8) : 1) 
         // below 2^-60 a row is zero in every use (fp16 ends at 2^-24) and its
         // reciprocal would leave fp32; an infinity or NaN marks the whole row
         const bool tiny = mx < 0x1p-60f, sound = mx <= 3.4028235e38f;
-        // mx / 127 rounded: a product and its residual step
+        // mx / 127 correctly rounded: the rounded reciprocal's product and its residual (Markstein, as above)
         const float s0 = mx * (1.f / 127.f), s1 = fmaf(fmaf(-127.f, s0, mx), 1.f / 127.f, s0);
         const bool coded = sound && !tiny;
         const float scale = coded ? s1 : 0.f, inv = coded ? rcp_approx(s1) : 0.f;
