@@ -25,6 +25,14 @@ import torch
 from . import _capi
 from ._capi import F16, F32, I8, I32, KllmError, check, lib
 
+try:  # without the Stream object and the lazy initialisation of the public functions: 1 us a call
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream, _cuda_getDevice as _current_device
+except ImportError:  # names that torch does not promise
+    def _raw_stream(index: int) -> int:
+        return torch.cuda.current_stream(index).cuda_stream
+
+    _current_device = torch.cuda.current_device
+
 _DTYPES = {torch.float32: F32, torch.float16: F16, torch.int32: I32, torch.int8: I8}
 
 
@@ -58,7 +66,7 @@ def _ptr(t):
 
 
 def _stream(device) -> int:
-    return torch._C._cuda_getCurrentRawStream(device.index)
+    return _raw_stream(device.index)
 
 
 def set_pdl(enable: bool) -> bool:
@@ -430,8 +438,8 @@ def _call(device, entry, *args) -> None:
     """Calls a C entry point with `device` current (the context is entered only
     when it is not) and its stream appended, and checks the status."""
     index = device.index
-    if index == torch._C._cuda_getDevice():
-        status = entry(*args, torch._C._cuda_getCurrentRawStream(index))
+    if index == _current_device():
+        status = entry(*args, _raw_stream(index))
     else:
         with torch.cuda.device(device):
             status = entry(*args, _stream(device))
@@ -639,7 +647,7 @@ def kv_read_paged(cache: PagedKVCache, positions: torch.Tensor, seqs: torch.Tens
 
 def attention_paged_workspace_bytes(n_tokens: int, n_heads: int, cache: PagedKVCache) -> int:
     n = ctypes.c_int64(0)
-    if cache.device.index == torch._C._cuda_getDevice():
+    if cache.device.index == _current_device():
         check(lib.kllm_b200_attention_paged_workspace_bytes(n_tokens, n_heads, cache.descriptor(), n))
     else:
         with torch.cuda.device(cache.device):
