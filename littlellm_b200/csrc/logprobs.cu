@@ -672,16 +672,22 @@ int cluster_shift_for(int64_t rows, int64_t vocab) {
   return c;
 }
 
+// KEEP_ALL: the CTA's `vectors` all fit in shared memory.
 template <typename T, bool KEEP_ALL>
-int launch_logprobs(const LogprobArgs& a, int cta_shift, int64_t kept, const LaunchOpts& o) {
+int launch_logprobs(const LogprobArgs& a, int cta_shift, int64_t vectors, const LaunchOpts& o) {
   auto kernel = token_logprobs_kernel<T, KEEP_ALL>;
-  cudaError_t err = allow_smem(reinterpret_cast<const void*>(kernel), kKeep * 16 + sizeof(Shared));
-  if (err != cudaSuccess) return launch_status(err, "token_logprobs: shared memory opt-in");
-  const size_t smem = a.top_k == 0 || !KEEP_ALL ? 0 : static_cast<size_t>(kept) * 16;
+  size_t smem = 0;
+  if constexpr (KEEP_ALL) {
+    // opted in to the most any call keeps: with the static part it passes the default 48 KB
+    const cudaError_t err = allow_smem(reinterpret_cast<const void*>(kernel), kKeep * 16 + sizeof(Shared));
+    if (err != cudaSuccess) return launch_status(err, "token_logprobs: shared memory opt-in");
+    if (a.top_k > 0) smem = static_cast<size_t>(vectors) * 16;
+  }
   const dim3 grid(static_cast<unsigned>(a.rows << cta_shift));
-  err = cta_shift == 0 ? launch(kernel, grid, dim3(kThreads), smem, o.stream, o.pdl, a, 0)
-                       : launch_clustered(kernel, grid, dim3(kThreads), smem, o.stream, o.pdl, 1 << cta_shift, a,
-                                          cta_shift);
+  const cudaError_t err =
+      cta_shift == 0 ? launch(kernel, grid, dim3(kThreads), smem, o.stream, o.pdl, a, 0)
+                     : launch_clustered(kernel, grid, dim3(kThreads), smem, o.stream, o.pdl, 1 << cta_shift, a,
+                                        cta_shift);
   return launch_status(err, "token_logprobs");
 }
 
@@ -689,8 +695,7 @@ template <typename T>
 int run_logprobs(const LogprobArgs& a, const LaunchOpts& o) {
   const int c = cluster_shift_for(a.rows, a.vocab);
   const int64_t vectors = ((a.vocab / Vec<T>::kN) >> c) + 1;  // of a CTA, at most
-  return vectors <= kKeep ? launch_logprobs<T, true>(a, c, vectors, o)
-                          : launch_logprobs<T, false>(a, c, kBatch * kThreads, o);
+  return vectors <= kKeep ? launch_logprobs<T, true>(a, c, vectors, o) : launch_logprobs<T, false>(a, c, vectors, o);
 }
 
 }  // namespace
