@@ -57,8 +57,9 @@
 // loads and joins); over 1001: 5.4.
 #include <math.h>
 
+#include "mma.cuh"
 #include "paged.cuh"
-#include "tcgen05.cuh"  // smem_u32
+#include "tcgen05.cuh"  // smem_u32, cluster_sync
 
 namespace kb {
 namespace {
@@ -115,26 +116,8 @@ __device__ __forceinline__ int tiles_per_part(const PagedAttnArgs& a, int all_ti
   return (all_tiles + clusters * a.cluster - 1) / (clusters * a.cluster);
 }
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, int src_bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
-}
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int src_bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ void ldsm_x4(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x4_trans(uint32_t (&r)[4], uint32_t addr) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(addr));
 }
 // Transpose of an 8 x 8 fp16 matrix held two elements of a row per lane.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
@@ -142,24 +125,15 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                         uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};\n"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// The same with c = a * b (no registers to clear first).
-__device__ __forceinline__ void mma16816_new(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                             uint32_t b0, uint32_t b1) {
+// c = a * b for one m16n8k16 tile (no registers to clear first).
+__device__ __forceinline__ void mma16816_new(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
       "{%10,%10,%10,%10};\n"
       : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
+// The same of int8, m16n8k32.
 __device__ __forceinline__ void mma16832_new(int (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
@@ -189,13 +163,6 @@ __device__ __forceinline__ void digits(const float (&x)[4], uint32_t (&w)[3]) {
   }
 }
 
-// The larger of two values, NaN when either is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // Codes of bytes 0 and 2 of `w` as an fp16 pair (bytes 1 and 3: shift by 8).
 __device__ __forceinline__ uint32_t codes_h2(uint32_t w) {
   const uint32_t bias = 0x64806480u;  // 1152, 1152
@@ -204,16 +171,6 @@ __device__ __forceinline__ uint32_t codes_h2(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&r);
 }
 
-// 2^x in one instruction (2 ulp; results below the normal range are 0).
-__device__ __forceinline__ float exp2_approx(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.aligned;\nbarrier.cluster.wait.aligned;\n" ::: "memory");
-}
 // Four floats in the shared memory of CTA `rank` of the cluster, at this CTA's
 // `local` (16-byte aligned).
 __device__ __forceinline__ float4 ld_peer(const float* local, uint32_t rank) {
@@ -508,8 +465,8 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
           ldsm_x4(b, smem_u32(sk + swz<kRow>(mt * 16 + (lane & 15), 2 * ks + (lane >> 4))));
 #pragma unroll
           for (int h = 0; h < NH; ++h) {
-            if (ks == 0) mma16816_new(s[mt][h], b[0], b[1], b[2], b[3], qb[h][ks][0][0], qb[h][ks][1][0]);
-            else mma16816(s[mt][h], b[0], b[1], b[2], b[3], qb[h][ks][0][0], qb[h][ks][1][0]);
+            if (ks == 0) mma16816_new(s[mt][h], b, qb[h][ks][0][0], qb[h][ks][1][0]);
+            else mma16816(s[mt][h], b, qb[h][ks][0][0], qb[h][ks][1][0]);
           }
         }
         f[mt][0] = f[mt][1] = sl2;
@@ -678,15 +635,15 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
         if (!I8) {
           ldsm_x4_trans(b, smem_u32(sv + swz<kRow>(mt * 16 + 8 * (mtx >> 1) + (lane & 7), 2 * kp + (mtx & 1))));
 #pragma unroll
-          for (int h = 0; h < NH; ++h) mma16816(o[h][kp], b[0], b[1], b[2], b[3], pb[mt][h][0], pb[mt][h][1]);
+          for (int h = 0; h < NH; ++h) mma16816(o[h][kp], b, pb[mt][h][0], pb[mt][h][1]);
         } else {
           ldsm_x4_trans(b, smem_u32(sv + swz<kRow>(mt * 16 + 8 * (mtx & 1) + (lane & 7), 2 * kp + (mtx >> 1))));
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const uint32_t a0 = codes_h2(b[2 * e]), a1 = codes_h2(b[2 * e] >> 8);
-            const uint32_t a2 = codes_h2(b[2 * e + 1]), a3 = codes_h2(b[2 * e + 1] >> 8);
+            const uint32_t codes[4] = {codes_h2(b[2 * e]), codes_h2(b[2 * e] >> 8), codes_h2(b[2 * e + 1]),
+                                       codes_h2(b[2 * e + 1] >> 8)};
 #pragma unroll
-            for (int h = 0; h < NH; ++h) mma16816(o[h][2 * kp + e], a0, a1, a2, a3, pb[mt][h][0], pb[mt][h][1]);
+            for (int h = 0; h < NH; ++h) mma16816(o[h][2 * kp + e], codes, pb[mt][h][0], pb[mt][h][1]);
           }
         }
       }

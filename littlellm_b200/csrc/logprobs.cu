@@ -39,7 +39,7 @@
 #include <math.h>
 
 #include "ops.cuh"
-#include "tcgen05.cuh"  // smem_u32
+#include "tcgen05.cuh"  // smem_u32, cluster_rank
 
 namespace kb {
 namespace {
@@ -80,20 +80,6 @@ constexpr uint32_t kOrderNegInf = 0x007fffffu;  // order_of(-inf)
 
 __device__ __forceinline__ unsigned long long entry_of(uint32_t order, uint32_t id) {
   return (static_cast<unsigned long long>(order) << 32) | (0xffffffffu - id);
-}
-
-// 2^x in one instruction (2 ulp; results below the normal range are 0).
-__device__ __forceinline__ float exp2_approx(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-// The larger of two values, NaN when either is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
 }
 
 // Terms below 2^kFloor are 0 as fp32; t ends there, so that the 0 of a -inf
@@ -205,9 +191,7 @@ struct Batch<__half> {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 x = __half22float2(CLAMP ? as_h2(r[i]) : __hmax2_nan(as_h2(r[i]), as_h2(0xfbfffbffu)));
-        unsigned long long t2;
-        asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(t2) : "l"(f32x2_pack(x.x, x.y)), "l"(scale), "l"(less));
-        add_terms<CLAMP>(t2, s2, w2);
+        add_terms<CLAMP>(f32x2_fma(f32x2_pack(x.x, x.y), scale, less), s2, w2);
       }
     }
   }
@@ -220,8 +204,8 @@ struct Batch<__half> {
       hi = max_nan(hi, kFloor);
     }
     const unsigned long long e2 = f32x2_pack(exp2_approx(lo), exp2_approx(hi));
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(s2) : "l"(s2), "l"(e2));
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(w2) : "l"(e2), "l"(f32x2_pack(lo, hi)), "l"(w2));
+    s2 = f32x2_add(s2, e2);
+    w2 = f32x2_fma(e2, f32x2_pack(lo, hi), w2);
   }
 };
 
@@ -264,11 +248,6 @@ struct Batch<float> {
 
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.aligned;\n" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.aligned;\n" ::: "memory"); }
-__device__ __forceinline__ uint32_t cluster_rank() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
 // Stores to the same shared variable of the cluster's first CTA.
 __device__ __forceinline__ uint32_t first_cta(const void* local) {
   uint32_t r;

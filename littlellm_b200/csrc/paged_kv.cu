@@ -76,24 +76,6 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return r;
 }
 
-__device__ __forceinline__ unsigned long long f32x2_fma(unsigned long long a, unsigned long long b, unsigned long long c) {
-  unsigned long long r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ unsigned long long f32x2_add(unsigned long long a, unsigned long long b) {
-  unsigned long long r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
-// The larger of two values, NaN when either is.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-
 // rint(x / scale) of eight values as codes, the quotient by Markstein's residual
 // correction (P. Markstein, Computation of elementary functions on the IBM RISC
 // System/6000 processor, 1990). inv is 1 / scale to an ulp or two, so q = x inv
