@@ -373,10 +373,12 @@ int kllm_b200_kv_read_paged(const kllm_b200_paged_cache* cache, const int32_t* p
  * kllm_b200_attention_head_major): out[t, h, :] = sum_j p_j * v_j over the
  * positions j = 0..positions[t] of sequence seqs[t], p = softmax_j(q[t, h, :] .
  * k_j / sqrt(head_dim)), kv head h / (n_heads / n_kv_heads). Scores, softmax
- * statistics and sums in fp32; the probabilities enter the product with v as
- * fp16. q and out fp16 with q_stride and out_stride elements between tokens
- * (multiples of 8), 16-byte aligned, not overlapping (out == q is refused). At most 16 query heads
- * per kv head. Each token is attended on its own (several tokens of one
+ * statistics and sums in fp32. The probabilities enter the product with v as
+ * two fp16 parts over F16 pages (22 bits: the error is that of rounding the
+ * result), as fp16 over I8 pages (up to 2^-11 each, a sixteenth of the codes' own
+ * step). q and out fp16 with q_stride and out_stride elements between tokens
+ * (multiples of 8), 16-byte aligned, not overlapping (out == q is refused). At
+ * most 16 query heads per kv head. Each token is attended on its own (several tokens of one
  * sequence are allowed; each reads the sequence's pages again). Rows of
  * padding or flagged tokens become zeros. A cached row beyond positions[t] is
  * never used, whatever it holds.

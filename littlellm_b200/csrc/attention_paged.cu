@@ -37,7 +37,18 @@
 // 11 bits as operands of the second product; for int8 rows, whose probabilities
 // carry the scale of the value, that scale is taken relative to a power of two
 // at or above the largest the warp has met. Scores, sums and accumulators are
-// fp32. Rescales and joins go by r itself: past 2^24 kLift no longer comes off
+// fp32.
+//
+// fp16 rows take the probabilities in two fp16 parts, 22 bits: with one, outputs
+// are off by 1.1 to 1.4 times what rounding the exact result to fp16 leaves (1.6
+// for single tokens), with two by 1.0. HBM hides the second part (2048 sequences
+// of up to 4095 positions, 309 us either way; short ones 1 to 2% slower, with
+// more than eight query heads a kv head 6%). int8 rows take one part: half a step
+// of the cached values themselves is up to 2^-8 of a row's largest, sixteen times
+// the rounding of the probabilities, and issue bounds this form (184 us, with two
+// parts 199).
+//
+// Rescales and joins go by r itself: past 2^24 kLift no longer comes off
 // the maximum exactly. While the largest score is below kFar, an exponent is one
 // FMA: the dot product times its factor, exact, minus r. Past that the product
 // is rounded first, as it is for the maximum: what that rounding leaves out
@@ -607,10 +618,14 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
       }
       powers();
     }
-    // P^T as B fragments: the transpose of each 8 x 8 block
-    uint32_t pb[2][NH][2];
+    // O^T += V^T P^T, for 16 positions at a time. P^T as B fragments is the
+    // transpose of each 8 x 8 block: [h][0..1] the powers rounded to fp16 and, for
+    // fp16 rows, [h][2..3] what that rounding left. fp16: m tile k holds dims
+    // 16 k + gid, + 8; int8: dims 16 k + 2 gid, 2 gid + 1 (the two codes of the
+    // 16-bit units transposed)
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
+      uint32_t pb[NH][I8 ? 2 : 4];
       float v0 = 1.f, v1 = 1.f;
       if (I8) {
         v0 = ss[kTile + mt * 16 + gid] * inv_vref;
@@ -620,22 +635,29 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
       for (int h = 0; h < NH; ++h) {
         l[h][0] += p[mt][h][0] + p[mt][h][2];
         l[h][1] += p[mt][h][1] + p[mt][h][3];
-        pb[mt][h][0] = transpose8x8(f2_to_h2(p[mt][h][0] * v0, p[mt][h][1] * v0));
-        pb[mt][h][1] = transpose8x8(f2_to_h2(p[mt][h][2] * v1, p[mt][h][3] * v1));
-      }
-    }
-    // O^T += V^T P^T. fp16: m tile k holds dims 16 k + gid, + 8; int8: dims
-    // 16 k + 2 gid, 2 gid + 1 (the two codes of the 16-bit units transposed)
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt) {
+        for (int half = 0; half < 2; ++half) {
+          const float v = half == 0 ? v0 : v1;
+          const float x = p[mt][h][2 * half] * v, y = p[mt][h][2 * half + 1] * v;
+          const uint32_t rounded = f2_to_h2(x, y);
+          pb[h][half] = transpose8x8(rounded);
+          if constexpr (!I8) {
+            const float2 kept = h2_to_f2(rounded);
+            pb[h][2 + half] = transpose8x8(f2_to_h2(x - kept.x, y - kept.y));
+          }
+        }
+      }
       const int mtx = lane >> 3;
 #pragma unroll
       for (int kp = 0; kp < (I8 ? kM / 2 : kM); ++kp) {
         uint32_t b[4];
-        if (!I8) {
+        if constexpr (!I8) {
           ldsm_x4_trans(b, smem_u32(sv + swz<kRow>(mt * 16 + 8 * (mtx >> 1) + (lane & 7), 2 * kp + (mtx & 1))));
 #pragma unroll
-          for (int h = 0; h < NH; ++h) mma16816(o[h][kp], b, pb[mt][h][0], pb[mt][h][1]);
+          for (int h = 0; h < NH; ++h) {
+            mma16816(o[h][kp], b, pb[h][0], pb[h][1]);
+            mma16816(o[h][kp], b, pb[h][2], pb[h][3]);
+          }
         } else {
           ldsm_x4_trans(b, smem_u32(sv + swz<kRow>(mt * 16 + 8 * (mtx & 1) + (lane & 7), 2 * kp + (mtx >> 1))));
 #pragma unroll
@@ -643,7 +665,7 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
             const uint32_t codes[4] = {codes_h2(b[2 * e]), codes_h2(b[2 * e] >> 8), codes_h2(b[2 * e + 1]),
                                        codes_h2(b[2 * e + 1] >> 8)};
 #pragma unroll
-            for (int h = 0; h < NH; ++h) mma16816(o[h][2 * kp + e], codes, pb[mt][h][0], pb[mt][h][1]);
+            for (int h = 0; h < NH; ++h) mma16816(o[h][2 * kp + e], codes, pb[h][0], pb[h][1]);
           }
         }
       }
