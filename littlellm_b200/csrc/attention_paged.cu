@@ -44,7 +44,7 @@
 // for single tokens), with two by 1.0. HBM hides the second part (2048 sequences
 // of up to 4095 positions, 309 us either way; short ones 1 to 2% slower, with
 // more than eight query heads a kv head 6%). int8 rows take one part: half a step
-// of the cached values themselves is up to 2^-8 of a row's largest, sixteen times
+// of the cached values themselves is up to 2^-8 of a row's largest, eight times
 // the rounding of the probabilities, and issue bounds this form (184 us, with two
 // parts 199).
 //
@@ -60,12 +60,14 @@
 // distributed shared memory (each takes a slice of the output), clusters
 // through the caller's workspace and a second kernel.
 //
-// Measured (B200, of the 6540 GB/s copy rate; all of a read-only stream), 14
-// heads over 2 kv heads of 64, pages of 16: 2048 sequences of 1 to 4095
-// positions fp16 309 us (1.07), int8 184 us (0.95; 1000 x 4096 positions 0.98).
-// 29 sequences of 77 to 4093, 32 heads of 128, int8: 79 us (0.99). One token
-// over 131072 positions, fp16: 17.3 us (0.59: about 6 us of dependent first
-// loads and joins); over 1001: 5.4.
+// Measured (several B200s, of the 6540 GB/s copy rate; all of a read-only
+// stream), 14 heads over 2 kv heads of 64, pages of 16, kernel alone at full
+// clock: 2048 sequences of 1 to 4095 positions fp16 309 to 315 us (1.05 to 1.07),
+// int8 183 to 206 us (0.85 to 0.96); a call, repeated until the power cap acts,
+// 312 to 321 and 203 to 219 us (0.80 to 0.87). 29 sequences of 77 to 4093, 32
+// heads of 128, int8: 79 to 80 us (0.98), a call 84 to 91. One token over 131072
+// positions, fp16: 17.1 to 17.6 us (0.59: about 6 us of dependent first loads and
+// joins); over 1001: 5.5 to 6.0.
 #include <math.h>
 
 #include "mma.cuh"
@@ -949,7 +951,10 @@ int check_heads(const char* what, int64_t n_tokens, int64_t n_heads, int64_t hkv
 // loads, the join), so there a CTA is one warp, with a quarter of the shared
 // memory and more than twice to seven times the CTAs per SM. By waves of the
 // four-warp form: the longer the sequences may be, the more waves it takes
-// until the device stays full to the end without several warps per item.
+// until the device stays full to the end without several warps per item. The
+// rule (items * kNarrow >= capacity * CTAs of a wave) goes by these sizes; at its
+// edge one warp is the slower by up to 3% (2000 items of 512, 16000 of 2048), and
+// past a capacity of 2048 it stands unmeasured.
 // Measured, us, four warps / one, lengths of a quarter to all of the capacity:
 //                          capacity 32      128         512         1024        2048
 //   fp16 14/2 x 64    2000 items 14 / 8     17 / 11     32 / 33     55 / 59     100 / 109

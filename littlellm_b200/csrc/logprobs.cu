@@ -27,15 +27,17 @@
 // 64-bit number, so equal values have one order whatever the schedule.
 //
 // A row is read by a cluster of 1 to 8 CTAs whose parts are pushed to the
-// first one's shared memory: one launch, no workspace. Bound: rows * vocab
-// values from HBM; one exponential per value (the special-function unit needs
-// three quarters of the time that fp16 values need from HBM), about seven
-// issue slots per value. 2048 x 151936 fp16: 106 us without entries (0.90 of
-// the copy rate), 116 us with 5 (4300 warp instructions a row: keeping batches,
-// the bound, the list); one row with 20: 7.9 us. Whole batches are loaded without
+// first one's shared memory: one launch, no workspace. Per value there are its
+// bytes from HBM, one exponential and 8.6 instructions (0.9 of them for five
+// entries: keeping batches, the bound, the list). For 2048 x 151936 fp16 that is
+// 95 us at the copy rate, 69 us of the special-function unit and 75 us of issue
+// at 1.9 GHz, 82 and 89 us at the 1.6 GHz that the power cap leaves a loop of
+// calls; the three do not overlap fully. Kernel alone at full clock 116 to 120 us
+// with 5 entries (0.79 to 0.82 of the copy rate), 106 without; a call, repeated,
+// 131 to 133 (0.72). One row with 20: 8 to 10 us. Whole batches are loaded without
 // predicates into two sets in turn (a copy of 16 registers and as many defaults
 // per batch less: 4%). CTAs that stay and load their next row's first batch while
-// they finish one took 131 us (spills).
+// they finish one took 131 us where these took 118 (spills).
 #include <math.h>
 
 #include "ops.cuh"

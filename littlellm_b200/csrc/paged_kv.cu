@@ -122,10 +122,10 @@ __device__ __forceinline__ void lds8(const float* p, float (&f)[8]) {
 // U sets of heads per warp. SHARED: every warp of the CTA works on the same
 // token, which computes its cos/sin once; else each warp computes its own
 // token's. Many tokens want warps more than registers: 16384 tokens of 96
-// heads of 128, int8, 148 us held to 9 CTAs per SM, 164 at the 7 that fit
-// unheld (103 us of HBM time; the rest is issue, about 290 instructions for
-// four heads, and the wait for a warp's first loads: CTAs that stay and load
-// their next token beside the present one took 188 us).
+// heads of 128, int8, 148 us held to 9 CTAs per SM (8 bytes spilled), 164 at the
+// 7 that fit unheld (103 us of HBM time; the rest is issue, about 290
+// instructions for four heads, and the wait for a warp's first loads: CTAs that
+// stay and load their next token beside the present one took 188 us).
 template <int D, bool I8, int U, bool SHARED>
 __global__ void __launch_bounds__(kThreads, SHARED && U > 1 ? (I8 ? 9 : 8) : 1) qkv_norm_rope_append_paged_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int L = D / 16;    // lanes of one head
