@@ -374,7 +374,7 @@ int kllm_b200_kv_read_paged(const kllm_b200_paged_cache* cache, const int32_t* p
  * positions j = 0..positions[t] of sequence seqs[t], p = softmax_j(q[t, h, :] .
  * k_j / sqrt(head_dim)), kv head h / (n_heads / n_kv_heads). Scores, softmax
  * statistics and sums in fp32. The probabilities enter the product with v as
- * two fp16 parts over F16 pages (22 bits: the error is that of rounding the
+ * two fp16 parts over F16 pages (21 bits: the error is that of rounding the
  * result), as fp16 over I8 pages (up to 2^-11 each, a sixteenth of the codes' own
  * step). q and out fp16 with q_stride and out_stride elements between tokens
  * (multiples of 8), 16-byte aligned, not overlapping (out == q is refused). At

@@ -39,7 +39,7 @@
 // at or above the largest the warp has met. Scores, sums and accumulators are
 // fp32.
 //
-// fp16 rows take the probabilities in two fp16 parts, 22 bits: with one, outputs
+// fp16 rows take the probabilities in two fp16 parts, 21 bits: with one, outputs
 // are off by 1.1 to 1.4 times what rounding the exact result to fp16 leaves (1.6
 // for single tokens), with two by 1.0. HBM hides the second part (2048 sequences
 // of up to 4095 positions, 309 us either way; short ones 1 to 2% slower, with
@@ -131,6 +131,12 @@ __device__ __forceinline__ int tiles_per_part(const PagedAttnArgs& a, int all_ti
 
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, int src_bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;\n" ::"r"(dst), "l"(src), "r"(src_bytes) : "memory");
+}
+// Two floats as an fp16 pair, rounded towards zero.
+__device__ __forceinline__ uint32_t f2_to_h2_down(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
 // Transpose of an 8 x 8 fp16 matrix held two elements of a row per lane.
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
@@ -621,10 +627,12 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
       powers();
     }
     // O^T += V^T P^T, for 16 positions at a time. P^T as B fragments is the
-    // transpose of each 8 x 8 block: [h][0..1] the powers rounded to fp16 and, for
-    // fp16 rows, [h][2..3] what that rounding left. fp16: m tile k holds dims
-    // 16 k + gid, + 8; int8: dims 16 k + 2 gid, 2 gid + 1 (the two codes of the
-    // 16-bit units transposed)
+    // transpose of each 8 x 8 block: for int8 rows the powers rounded to fp16; for
+    // fp16 rows [h][0..1] the powers rounded towards zero and [h][2..3] what that
+    // left, 2^-24 (fp16's smallest, 2^-35 of the largest power) at least: neither
+    // negative nor zero, so that an infinite value stays that infinity. fp16: m tile
+    // k holds dims 16 k + gid, + 8; int8: dims 16 k + 2 gid, 2 gid + 1 (the two codes
+    // of the 16-bit units transposed)
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
       uint32_t pb[NH][I8 ? 2 : 4];
@@ -641,11 +649,13 @@ attn_paged_kernel(const __grid_constant__ PagedAttnArgs a) {
         for (int half = 0; half < 2; ++half) {
           const float v = half == 0 ? v0 : v1;
           const float x = p[mt][h][2 * half] * v, y = p[mt][h][2 * half + 1] * v;
-          const uint32_t rounded = f2_to_h2(x, y);
-          pb[h][half] = transpose8x8(rounded);
-          if constexpr (!I8) {
-            const float2 kept = h2_to_f2(rounded);
-            pb[h][2 + half] = transpose8x8(f2_to_h2(x - kept.x, y - kept.y));
+          if constexpr (I8) {
+            pb[h][half] = transpose8x8(f2_to_h2(x, y));
+          } else {
+            const uint32_t most_of = f2_to_h2_down(x, y);
+            const float2 kept = h2_to_f2(most_of);
+            pb[h][half] = transpose8x8(most_of);
+            pb[h][2 + half] = transpose8x8(f2_to_h2(fmaxf(x - kept.x, 0x1p-24f), fmaxf(y - kept.y, 0x1p-24f)));
           }
         }
       }
