@@ -42,11 +42,11 @@
 // fp16 rows take the probabilities in two fp16 parts, 21 bits: with one, outputs
 // are off by 1.1 to 1.4 times what rounding the exact result to fp16 leaves (1.6
 // for single tokens), with two by 1.0. HBM hides the second part (2048 sequences
-// of up to 4095 positions, 309 us either way; short ones 1 to 2% slower, with
-// more than eight query heads a kv head 6%). int8 rows take one part: half a step
-// of the cached values themselves is up to 2^-8 of a row's largest, eight times
-// the rounding of the probabilities, and issue bounds this form (184 us, with two
-// parts 199).
+// of up to 4095 positions, 312 / 315 us with one / two; short ones 1 to 4% slower,
+// with more than eight query heads a kv head 5 to 8%). int8 rows take one part:
+// half a step of the cached values themselves is up to 2^-8 of a row's largest,
+// eight times the rounding of the probabilities, and issue bounds this form (184
+// us, with two parts 199).
 //
 // Rescales and joins go by r itself: past 2^24 kLift no longer comes off
 // the maximum exactly. While the largest score is below kFar, an exponent is one
